@@ -512,6 +512,73 @@ int mdlm_adamw_ema(float* p, const float* g, float* m, float* v, float* ema,
                    float ema_one_minus_decay, const float* sumsq, float max_norm,
                    float grad_scale, void* stream);
 
+/* Scores of the SUBS rows (diffusion.py:261-277) without the (rows, V) table; no
+ * reference counterpart.  With l the row of log-probabilities of
+ * mdlm_subs_logprobs:
+ *   logp[r]     = l[x0[r]]  (x0 outside [0, V): no token there, 0)
+ *   entropy[r]  = -sum_v e^{l_v} l_v        (0 log 0 = 0)
+ *   lse[r]      = log-sum-exp of the logits, mask column excluded
+ *   top_ids, top_logp (rows, top_k): the columns with the largest logits, the
+ *     mask column excluded, best first, equal logits by index (NaN counts as
+ *     largest), and their l.  0 <= top_k <= 64, top_k < V; 0: not computed.
+ * A row with xt != mask_index is known and not read: logp is 0 for x0 == xt and
+ * -1e6 otherwise, entropy and lse are 0, the alternatives are xt (0) and the lowest
+ * other indices (-1e6).  A masked row without a finite logit, or with a NaN or
+ * +inf outside the mask column, has no distribution: its scores are NaN (lse -inf
+ * where every logit is -inf).
+ * logits fp32 or bf16, rows `ld` elements apart, aligned to their type.  ws: of
+ * mdlm_subs_scores_workspace_bytes (NULL where that is 0); calls that overlap in
+ * time need one each. */
+int mdlm_subs_scores(const void* logits, int64_t ld, int dtype,
+                     const int64_t* xt, const int64_t* x0, float* logp,
+                     float* entropy, float* lse, float* top_logp,
+                     int64_t* top_ids, int64_t rows, int V, int mask_index,
+                     int top_k, void* ws, void* stream);
+
+/* Gradient of mdlm_subs_scores with respect to the logits, in their type: lse,
+ * entropy, top_ids (rows, top_k) as it left them; g_logp, g_entropy (rows) and
+ * g_top (rows, top_k) are the incoming gradients (the first two may be NULL:
+ * zero).  Zero for known rows, in the mask column and in rows whose incoming
+ * gradients are all zero (whatever their logits hold).  An index outside [0, V)
+ * takes no gradient; one that occurs twice takes both.  Columns from V to ldo are not written.
+ * dlogits may be the logits themselves. */
+int mdlm_subs_scores_bwd(const void* logits, int64_t ld, int dtype,
+                         const int64_t* xt, const int64_t* x0, const float* lse,
+                         const float* entropy, const float* g_logp,
+                         const float* g_entropy, const int64_t* top_ids,
+                         const float* g_top, int top_k, void* dlogits,
+                         int64_t ldo, int64_t rows, int V, int mask_index,
+                         void* stream);
+
+/* Orthogonalised matrices: X = G / (|G|_F + eps), then `steps` times
+ * X <- a X + (b A + c A^2) X with A = X X^T (X^T X for a tall G): singular values
+ * go towards 1, singular vectors stay.  No reference counterpart (its optimizer
+ * is AdamW, diffusion.py:449-459).  n matrices (rows, cols), fp32 or bf16, rows
+ * `ld` and matrices `stride` elements apart; out bf16 (the products round their
+ * operands to fp16: the result is good to bf16).  c != 0, |b / 2c| <= 8.
+ * ws: mdlm_orthogonalize_workspace_bytes(n, rows, cols), 256-byte aligned. */
+int mdlm_orthogonalize(const void* g, int64_t ldg, int64_t g_stride, int dtype,
+                       void* out_bf16, int64_t ldo, int64_t out_stride, int n,
+                       int rows, int cols, int steps, double a, double b,
+                       double c, double eps, void* ws, void* stream);
+
+/* One optimizer step of n weight matrices by orthogonalised momentum, the
+ * counterpart of mdlm_adamw_ema (same clipping, decay, moving average and bf16
+ * copy) for 2-D weights:
+ *   g <- g * grad_scale * min(1, max_norm / (norm + 1e-6))    (as mdlm_adamw_ema)
+ *   m <- m + (1 - momentum) (g - m)
+ *   O  = orthogonalize(g + momentum (m - g))
+ *   p <- p (1 - lr weight_decay) - lr update_scale O
+ * p, g, m, ema (may be NULL): fp32, w_bf16 (may be NULL): bf16, all of the same
+ * layout (rows `ld`, matrices `stride` elements apart).  g is not written.
+ * ws: mdlm_orthogonalize_workspace_bytes(n, rows, cols), 256-byte aligned. */
+int mdlm_muon_update(float* p, const float* g, float* m, float* ema,
+                     void* w_bf16, int64_t ld, int64_t stride, int n, int rows,
+                     int cols, float lr, float momentum, float weight_decay,
+                     float update_scale, int steps, double a, double b, double c,
+                     double eps, float ema_one_minus_decay, const float* sumsq,
+                     float max_norm, float grad_scale, void* ws, void* stream);
+
 /* ------------------------------------------------------- workspace sizes
  * SURVEY 8(b) "Ownership": the caller allocates every buffer and sizes the
  * workspaces with these queries (host arithmetic only; bytes, or -1 for a bad
@@ -523,7 +590,11 @@ int mdlm_adamw_ema(float* p, const float* g, float* m, float* v, float* ema,
  *   embed_grad          : hot_partial
  *   ln_modulate_bwd, dropout_gate_residual_bwd, colsum_bf16_partial : partial
  *   transpose_bf16      : colsum_partial
- *   masked_row_map      : gather and scatter, each (rows = B*L) */
+ *   masked_row_map      : gather and scatter, each (rows = B*L)
+ *   subs_scores         : ws (0: none needed)
+ *   orthogonalize       : ws of orthogonalize and muon_update */
+int64_t mdlm_subs_scores_workspace_bytes(int64_t rows, int V, int top_k);
+int64_t mdlm_orthogonalize_workspace_bytes(int n, int rows, int cols);
 int64_t mdlm_attn_bwd_workspace_bytes(int n_seq, int H, int L);
 int64_t mdlm_grad_sumsq_workspace_bytes(void);
 int64_t mdlm_gemm_bf16_splitk_workspace_bytes(int64_t M, int N, int splits);

@@ -4,6 +4,9 @@ PyTorch is plumbing here: it owns device memory and the stream; all arithmetic
 runs in the hand-written HIP kernels.  Every wrapper requires CUDA (ROCm)
 tensors and raises otherwise -- there is no CPU path.
 """
+import math
+from typing import NamedTuple, Optional
+
 import torch
 
 from . import _lib
@@ -648,3 +651,170 @@ def adamw_ema(p, g, m, v, ema, w16, lr, beta1, beta2, eps, weight_decay, step,
        _p(ema), _p(w16), p.numel(), float(lr), float(beta1), float(beta2),
        float(eps), float(weight_decay), int(step), float(ema_one_minus_decay),
        _p(sumsq), float(max_norm), float(grad_scale), _stream())
+
+
+# ------------------------------------------------------------- token scores
+class SubsScores(NamedTuple):
+  """Result of `subs_scores`: (...) fp32, and (..., top_k) fp32 / int64 (None for top_k = 0)."""
+  logp: torch.Tensor
+  entropy: torch.Tensor
+  lse: torch.Tensor
+  top_logp: Optional[torch.Tensor]
+  top_ids: Optional[torch.Tensor]
+
+
+def _same_device(ref, **tensors):
+  for name, t in tensors.items():
+    if t is not None and _dev(t, name).device != ref.device:
+      raise RuntimeError(f'{name}: on {t.device}, expected {ref.device}')
+
+
+def _row_vec(t, name, logits, dtype):
+  """One value per row of `logits`, contiguous."""
+  t = _dev(t, name, dtype)
+  if t.shape != logits.shape[:-1]:
+    raise RuntimeError(f'{name}: shape {tuple(t.shape)}, expected {tuple(logits.shape[:-1])}')
+  return t.contiguous()
+
+
+def subs_scores(logits, xt, x0, mask_index, top_k=0):
+  """Log-probability of the tokens x0, entropy, log-sum-exp and the top_k best
+  alternatives of every SUBS row, without the (rows, V) table (see
+  mdlm_subs_scores in include/mdlm_hip.h).  logits (rows, V) or (B, L, V)."""
+  lg, rows, V, ld = _rows2d(logits, 'logits')
+  _same_device(lg, xt=xt, x0=x0)
+  xt = _row_vec(xt, 'xt', logits, torch.int64)
+  x0 = _row_vec(x0, 'x0', logits, torch.int64)
+  k = int(top_k)
+  if k < 0 or k > 64 or (k and k >= V):
+    raise RuntimeError(f'top_k={k}: must be in 0..64 and less than V={V}')
+  with torch.cuda.device(lg.device):
+    f = torch.empty((3,) + tuple(xt.shape), dtype=torch.float32, device=lg.device)
+    tl = ti = ws = None
+    if k:
+      tl = torch.empty(tuple(xt.shape) + (k,), dtype=torch.float32, device=lg.device)
+      ti = torch.empty(tuple(xt.shape) + (k,), dtype=torch.int64, device=lg.device)
+    nbytes = workspace_bytes('subs_scores', rows, V, k)
+    if nbytes:
+      ws = torch.empty(nbytes, dtype=torch.uint8, device=lg.device)
+    call('mdlm_subs_scores', lg.data_ptr(), ld, _DT[lg.dtype], xt.data_ptr(), x0.data_ptr(),
+         f[0].data_ptr(), f[1].data_ptr(), f[2].data_ptr(), _p(tl), _p(ti), rows, V,
+         int(mask_index), k, _p(ws), _stream())
+  return SubsScores(f[0], f[1], f[2], tl, ti)
+
+
+def subs_scores_bwd(logits, xt, x0, mask_index, lse, entropy, g_logp=None, g_entropy=None,
+                    top_ids=None, g_top=None, dlogits=None):
+  """Gradient of `subs_scores` with respect to the logits (their dtype).  `dlogits`:
+  written if given (may be `logits` itself); columns past V are left alone."""
+  lg, rows, V, ld = _rows2d(logits, 'logits')
+  _same_device(lg, xt=xt, x0=x0, lse=lse, entropy=entropy, g_logp=g_logp, g_entropy=g_entropy,
+               top_ids=top_ids, g_top=g_top, dlogits=dlogits)
+  xt = _row_vec(xt, 'xt', logits, torch.int64)
+  x0 = _row_vec(x0, 'x0', logits, torch.int64)
+  lse = _row_vec(lse, 'lse', logits, torch.float32)
+  entropy = _row_vec(entropy, 'entropy', logits, torch.float32)
+  if g_logp is not None:
+    g_logp = _row_vec(g_logp, 'g_logp', logits, torch.float32)
+  if g_entropy is not None:
+    g_entropy = _row_vec(g_entropy, 'g_entropy', logits, torch.float32)
+  k = 0
+  if g_top is not None:
+    k = g_top.shape[-1]
+    if top_ids is None or top_ids.shape != g_top.shape or g_top.shape[:-1] != logits.shape[:-1]:
+      raise RuntimeError('g_top: needs top_ids of the same shape, one row per row of logits')
+    if k > 64 or (k and k >= V):
+      raise RuntimeError(f'g_top: {k} alternatives, at most 64 and less than V={V}')
+    g_top = _dev(g_top, 'g_top', torch.float32).contiguous()
+    top_ids = _dev(top_ids, 'top_ids', torch.int64).contiguous()
+  with torch.cuda.device(lg.device):
+    if dlogits is None:
+      if logits.dim() == 3:
+        dlogits = alloc_logits(logits.shape[0], logits.shape[1], V, lg.dtype, lg.device)
+      else:
+        dlogits = torch.empty(rows, padded_vocab(V), dtype=lg.dtype, device=lg.device)[:, :V]
+    o, orows, oV, ldo = _rows2d(dlogits, 'dlogits')
+    if o.dtype != lg.dtype or dlogits.shape != logits.shape:
+      raise RuntimeError(f'dlogits: expected {tuple(logits.shape)} {lg.dtype}, got {tuple(dlogits.shape)} {o.dtype}')
+    call('mdlm_subs_scores_bwd', lg.data_ptr(), ld, _DT[lg.dtype], xt.data_ptr(), x0.data_ptr(),
+         lse.data_ptr(), entropy.data_ptr(), _p(g_logp), _p(g_entropy), _p(top_ids) if k else 0,
+         _p(g_top) if k else 0, k, o.data_ptr(), ldo, rows, V, int(mask_index), _stream())
+  return dlogits
+
+
+# ------------------------------------------- orthogonalised weight update
+MUON_COEFFS = (3.4445, -4.7750, 2.0315)
+
+
+def _matrices(t, name, dtypes):
+  """(n, rows, cols, row stride, matrix stride) of a (rows, cols) or (n, rows, cols) tensor."""
+  _dev(t, name)
+  if t.dtype not in dtypes:
+    raise RuntimeError(f'{name}: dtype {t.dtype} not supported')
+  if t.dim() not in (2, 3):
+    raise RuntimeError(f'{name}: expected a (rows, cols) or (n, rows, cols) tensor')
+  r, c = t.shape[-2:]
+  if c > 1 and t.stride(-1) != 1:
+    raise RuntimeError(f'{name}: innermost dimension must be contiguous')
+  ld = t.stride(-2) if r > 1 else c
+  n = t.shape[0] if t.dim() == 3 else 1
+  bs = t.stride(0) if t.dim() == 3 and n > 1 else 0
+  return n, r, c, ld, bs
+
+
+def orthogonalize(g, steps=5, coeffs=MUON_COEFFS, eps=1e-7, out=None, ws=None):
+  """Newton-Schulz orthogonalisation of a matrix or a stack of matrices (bf16
+  result; see mdlm_orthogonalize in include/mdlm_hip.h).  ws: a workspace of
+  `workspace('orthogonalize', n, rows, cols)`, allocated if not given."""
+  n, r, c, ld, bs = _matrices(g, 'g', _DT)
+  _same_device(g, out=out, ws=ws)
+  with torch.cuda.device(g.device):
+    if out is None:
+      out = torch.empty(g.shape, dtype=torch.bfloat16, device=g.device)
+    if out.shape != g.shape:
+      raise RuntimeError(f'out: shape {tuple(out.shape)}, expected {tuple(g.shape)}')
+    _, _, _, ldo, bso = _matrices(out, 'out', (torch.bfloat16,))
+    if g.numel():
+      ws = _ortho_ws(ws, n, r, c, g.device)
+      call('mdlm_orthogonalize', g.data_ptr(), ld, bs, _DT[g.dtype], out.data_ptr(), ldo, bso, n, r, c,
+           int(steps), float(coeffs[0]), float(coeffs[1]), float(coeffs[2]), float(eps), ws.data_ptr(), _stream())
+  return out
+
+
+def _ortho_ws(ws, n, r, c, device):
+  need = workspace_bytes('orthogonalize', n, r, c)
+  if ws is None:
+    return torch.empty(need, dtype=torch.uint8, device=device)
+  if not ws.is_contiguous() or ws.numel() * ws.element_size() < need:
+    raise RuntimeError(f'ws: {ws.numel() * ws.element_size()} bytes, {need} needed')
+  return ws
+
+
+def muon_update(p, g, m, lr, ema=None, w16=None, momentum=0.95, weight_decay=0.0, scale=None,
+                steps=5, coeffs=MUON_COEFFS, eps=1e-7, sumsq=None, max_norm=0.0, grad_scale=1.0,
+                ema_one_minus_decay=0.0, ws=None):
+  """One optimizer step of a weight matrix (or a stack of them) by orthogonalised
+  momentum, in place on p, m, ema and w16 (see mdlm_muon_update in
+  include/mdlm_hip.h).  scale: of the orthogonal factor; None: 0.2 sqrt(max(rows,
+  cols)), which gives the update AdamW's usual size, so its learning rate carries
+  over.  sumsq, max_norm, grad_scale: clipping as in `adamw_ema`."""
+  n, r, c, ld, bs = _matrices(p, 'p', (torch.float32,))
+  _same_device(p, g=g, m=m, ema=ema, w16=w16, sumsq=sumsq, ws=ws)
+  for name, t in (('g', g), ('m', m), ('ema', ema), ('w16', w16)):
+    if t is None:
+      continue
+    got = _matrices(t, name, (torch.bfloat16 if name == 'w16' else torch.float32,))
+    if t.shape != p.shape or got != (n, r, c, ld, bs):
+      raise RuntimeError(f'{name}: must have the shape and strides of p')
+  if sumsq is not None:
+    _dev(sumsq, 'sumsq', torch.float32)
+  if scale is None:
+    scale = 0.2 * math.sqrt(max(r, c))
+  if p.numel():
+    with torch.cuda.device(p.device):
+      ws = _ortho_ws(ws, n, r, c, p.device)
+      call('mdlm_muon_update', p.data_ptr(), g.data_ptr(), m.data_ptr(), _p(ema), _p(w16), ld, bs, n, r, c,
+           float(lr), float(momentum), float(weight_decay), float(scale), int(steps), float(coeffs[0]),
+           float(coeffs[1]), float(coeffs[2]), float(eps), float(ema_one_minus_decay), _p(sumsq),
+           float(max_norm), float(grad_scale), ws.data_ptr(), _stream())
+  return p
