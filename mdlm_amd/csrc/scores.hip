@@ -211,7 +211,9 @@ __global__ __launch_bounds__(BLOCK) void subs_scores_kernel(
     const T* __restrict__ logits, int64_t ld, const int64_t* __restrict__ xt, const int64_t* __restrict__ x0,
     float* __restrict__ logp, float* __restrict__ ent, float* __restrict__ lse, float* __restrict__ top_logp,
     int64_t* __restrict__ top_ids, int V, int mask, int k) {
-  constexpr int E = RowSpan<T>::E, U = 4;
+  // chunks in flight per thread: a whole row of the common vocabularies for the wide
+  // workgroup, whose latency counts; the narrow ones hide theirs behind each other
+  constexpr int E = RowSpan<T>::E, U = BLOCK == 1024 ? 8 : 4;
   __shared__ ScoreShared<BLOCK> sh;
   const int64_t r = blockIdx.x;
   const int tid = threadIdx.x, w = tid >> 6;
@@ -236,15 +238,13 @@ __global__ __launch_bounds__(BLOCK) void subs_scores_kernel(
     }
     run.add(f);
   };
-  int i = tid;
-  for (; i + (U - 1) * BLOCK < sp.n; i += U * BLOCK) {
+  for (int i = tid; i < sp.n; i += U * BLOCK) {
     uint4 q[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) q[u] = chunks[i + u * BLOCK];
+    for (int u = 0; u < U; ++u) if (i + u * BLOCK < sp.n) q[u] = chunks[i + u * BLOCK];
 #pragma unroll
-    for (int u = 0; u < U; ++u) add_chunk(q[u], i + u * BLOCK);
+    for (int u = 0; u < U; ++u) if (i + u * BLOCK < sp.n) add_chunk(q[u], i + u * BLOCK);
   }
-  for (; i < sp.n; i += BLOCK) add_chunk(chunks[i], i);
   const int alone = tid < sp.head + sp.tail ? sp.single(tid) : -1;
   if (alone >= 0 && alone != mask) {
     const float f[1] = {elem<T>::load(row + alone)};
@@ -339,16 +339,16 @@ __global__ __launch_bounds__(BLOCK) void subs_scores_kernel(
 //   d_v = -p_v (total + gH (l_v + H)) = -2^t (g0 + g1 t)
 // and then the columns that take a gradient of their own (the given token, the
 // alternatives), each written once with all that it takes.
-template <typename T>
-__global__ __launch_bounds__(256) void subs_scores_bwd_kernel(
+template <typename T, int BLOCK>
+__global__ __launch_bounds__(BLOCK) void subs_scores_bwd_kernel(
     const T* logits, int64_t ld, const int64_t* __restrict__ xt, const int64_t* __restrict__ x0,
     const float* __restrict__ lse, const float* __restrict__ ent, const float* __restrict__ g_logp,
     const float* __restrict__ g_ent, const int64_t* __restrict__ top_ids, const float* __restrict__ g_top, int k,
     T* dl, int64_t ldo, int V, int mask) {
-  constexpr int E = RowSpan<T>::E, U = 4, BLOCK = 256;
+  constexpr int E = RowSpan<T>::E, U = BLOCK == 1024 ? 8 : 4;
   __shared__ float sg[SC_MAX_K + 1], sx[SC_MAX_K + 1];
   __shared__ int sid[SC_MAX_K + 1];
-  __shared__ float red[2][4];
+  __shared__ float red[2][BLOCK / 64];
   const int64_t r = blockIdx.x;
   const int tid = threadIdx.x;
   const bool live = xt[r] == mask;
@@ -387,13 +387,15 @@ __global__ __launch_bounds__(256) void subs_scores_bwd_kernel(
     m = wave_max(m);
     if ((tid & 63) == 0) red[0][tid >> 6] = m;
     __syncthreads();
-    m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    for (int j = 0; j < BLOCK / 64; ++j) m = fmaxf(m, red[0][j]);
     for (int v = tid; v < V; v += BLOCK)
       if (v != mask) lz += __builtin_amdgcn_exp2f((elem<T>::load(row + v) - m) * SC_L2E);
     lz = wave_sum(lz);
     if ((tid & 63) == 0) red[1][tid >> 6] = lz;
     __syncthreads();
-    lz = log2f((red[1][0] + red[1][1]) + (red[1][2] + red[1][3])) * SC_LN2;
+    lz = 0.f;
+    for (int j = 0; j < BLOCK / 64; ++j) lz += red[1][j];
+    lz = log2f(lz) * SC_LN2;
   }
   const float g0 = total + gh * H, g1 = gh * SC_LN2, l2z = lz * SC_L2E;
   const bool bad = !(fabsf(m) < INFINITY) || !(fabsf(lz) < INFINITY);    // no distribution: NaN
@@ -419,15 +421,13 @@ __global__ __launch_bounds__(256) void subs_scores_bwd_kernel(
   };
   const T* in = row + sp.head;
   auto pass = [&](auto load) {
-    int i = tid;
-    for (; i + (U - 1) * BLOCK < sp.n; i += U * BLOCK) {
+    for (int i = tid; i < sp.n; i += U * BLOCK) {
       uint4 q[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) q[u] = load(i + u * BLOCK);
+      for (int u = 0; u < U; ++u) if (i + u * BLOCK < sp.n) q[u] = load(i + u * BLOCK);
 #pragma unroll
-      for (int u = 0; u < U; ++u) do_chunk(q[u], i + u * BLOCK);
+      for (int u = 0; u < U; ++u) if (i + u * BLOCK < sp.n) do_chunk(q[u], i + u * BLOCK);
     }
-    for (; i < sp.n; i += BLOCK) do_chunk(load(i), i);
   };
   if (alone >= 0) elem<T>::store(out + alone, alone == mask ? 0.f : dense(elem<T>::load(row + alone)));
   if (((uintptr_t)in & 15) == 0) {
@@ -489,10 +489,12 @@ extern "C" int mdlm_subs_scores_bwd(const void* logits, int64_t ld, int dtype, c
   MDLM_CHECK_ARG(top_k >= 0 && top_k <= SC_MAX_K && top_k < V,
                  "subs_scores_bwd: top_k=%d must be at most %d and less than V=%d", top_k, SC_MAX_K, V);
   MDLM_CHECK_ARG(top_k == 0 || (top_ids && g_top), "subs_scores_bwd: null pointer (alternatives)");
-  if (dtype == MDLM_BF16)
-    subs_scores_bwd_kernel<bf16_t><<<(unsigned)rows, 256, 0, (hipStream_t)stream>>>((const bf16_t*)logits, ld, xt, x0, lse, entropy, g_logp, g_entropy, top_ids, g_top, top_k, (bf16_t*)dlogits, ldo, V, mask_index);
-  else if (dtype == MDLM_F32)
-    subs_scores_bwd_kernel<float><<<(unsigned)rows, 256, 0, (hipStream_t)stream>>>((const float*)logits, ld, xt, x0, lse, entropy, g_logp, g_entropy, top_ids, g_top, top_k, (float*)dlogits, ldo, V, mask_index);
+#define SC_LAUNCH(T, B) \
+  subs_scores_bwd_kernel<T, B><<<(unsigned)rows, B, 0, (hipStream_t)stream>>>((const T*)logits, ld, xt, x0, lse, entropy, g_logp, g_entropy, top_ids, g_top, top_k, (T*)dlogits, ldo, V, mask_index)
+  const bool wide = rows <= SC_WIDE_ROWS;
+  if (dtype == MDLM_BF16) { if (wide) SC_LAUNCH(bf16_t, 1024); else SC_LAUNCH(bf16_t, 256); }
+  else if (dtype == MDLM_F32) { if (wide) SC_LAUNCH(float, 1024); else SC_LAUNCH(float, 256); }
+#undef SC_LAUNCH
   else { set_error("subs_scores_bwd: bad dtype %d", dtype); return -1; }
   MDLM_LAUNCH_CHECK();
   return 0;

@@ -664,17 +664,38 @@ class SubsScores(NamedTuple):
 
 
 def _same_device(ref, **tensors):
+  dev = ref.device
   for name, t in tensors.items():
-    if t is not None and _dev(t, name).device != ref.device:
-      raise RuntimeError(f'{name}: on {t.device}, expected {ref.device}')
+    if t is not None and _dev(t, name).device != dev:
+      raise RuntimeError(f'{name}: on {t.device}, expected {dev}')
 
 
-def _row_vec(t, name, logits, dtype):
-  """One value per row of `logits`, contiguous."""
-  t = _dev(t, name, dtype)
-  if t.shape != logits.shape[:-1]:
-    raise RuntimeError(f'{name}: shape {tuple(t.shape)}, expected {tuple(logits.shape[:-1])}')
-  return t.contiguous()
+class _on_device:
+  """The device of `t` current inside, if it is not (entering torch.cuda.device costs
+  more than a small kernel); gives that device's current stream."""
+
+  def __init__(self, t):
+    self.index = t.get_device()
+
+  def __enter__(self):
+    self.prev = torch._C._cuda_getDevice()
+    if self.prev != self.index:
+      torch.cuda.set_device(self.index)
+    return torch._C._cuda_getCurrentRawStream(self.index)
+
+  def __exit__(self, *exc):
+    if self.prev != self.index:
+      torch.cuda.set_device(self.prev)
+
+
+def _row_vec(t, name, shape, dev, dtype):
+  """One value per row, contiguous, on the logits' device."""
+  _dev(t, name, dtype)
+  if t.get_device() != dev:
+    raise RuntimeError(f'{name}: on {t.device}, expected cuda:{dev}')
+  if t.shape != shape:
+    raise RuntimeError(f'{name}: shape {tuple(t.shape)}, expected {tuple(shape)}')
+  return t if t.is_contiguous() else t.contiguous()
 
 
 def subs_scores(logits, xt, x0, mask_index, top_k=0):
@@ -682,25 +703,25 @@ def subs_scores(logits, xt, x0, mask_index, top_k=0):
   alternatives of every SUBS row, without the (rows, V) table (see
   mdlm_subs_scores in include/mdlm_hip.h).  logits (rows, V) or (B, L, V)."""
   lg, rows, V, ld = _rows2d(logits, 'logits')
-  _same_device(lg, xt=xt, x0=x0)
-  xt = _row_vec(xt, 'xt', logits, torch.int64)
-  x0 = _row_vec(x0, 'x0', logits, torch.int64)
+  shape, dev = logits.shape[:-1], lg.get_device()
+  xt = _row_vec(xt, 'xt', shape, dev, torch.int64)
+  x0 = _row_vec(x0, 'x0', shape, dev, torch.int64)
   k = int(top_k)
   if k < 0 or k > 64 or (k and k >= V):
     raise RuntimeError(f'top_k={k}: must be in 0..64 and less than V={V}')
-  with torch.cuda.device(lg.device):
-    f = torch.empty((3,) + tuple(xt.shape), dtype=torch.float32, device=lg.device)
+  with _on_device(lg) as stream:
+    logp, ent, lse = torch.empty((3, *shape), dtype=torch.float32, device=lg.device).unbind(0)
     tl = ti = ws = None
     if k:
-      tl = torch.empty(tuple(xt.shape) + (k,), dtype=torch.float32, device=lg.device)
-      ti = torch.empty(tuple(xt.shape) + (k,), dtype=torch.int64, device=lg.device)
-    nbytes = workspace_bytes('subs_scores', rows, V, k)
-    if nbytes:
+      tl = torch.empty((*shape, k), dtype=torch.float32, device=lg.device)
+      ti = torch.empty((*shape, k), dtype=torch.int64, device=lg.device)
+    nbytes = _lib.call_i64('mdlm_subs_scores_workspace_bytes', rows, V, k)
+    if nbytes > 0:
       ws = torch.empty(nbytes, dtype=torch.uint8, device=lg.device)
     call('mdlm_subs_scores', lg.data_ptr(), ld, _DT[lg.dtype], xt.data_ptr(), x0.data_ptr(),
-         f[0].data_ptr(), f[1].data_ptr(), f[2].data_ptr(), _p(tl), _p(ti), rows, V,
-         int(mask_index), k, _p(ws), _stream())
-  return SubsScores(f[0], f[1], f[2], tl, ti)
+         logp.data_ptr(), ent.data_ptr(), lse.data_ptr(), _p(tl), _p(ti), rows, V,
+         int(mask_index), k, _p(ws), stream)
+  return SubsScores(logp, ent, lse, tl, ti)
 
 
 def subs_scores_bwd(logits, xt, x0, mask_index, lse, entropy, g_logp=None, g_entropy=None,
@@ -708,37 +729,37 @@ def subs_scores_bwd(logits, xt, x0, mask_index, lse, entropy, g_logp=None, g_ent
   """Gradient of `subs_scores` with respect to the logits (their dtype).  `dlogits`:
   written if given (may be `logits` itself); columns past V are left alone."""
   lg, rows, V, ld = _rows2d(logits, 'logits')
-  _same_device(lg, xt=xt, x0=x0, lse=lse, entropy=entropy, g_logp=g_logp, g_entropy=g_entropy,
-               top_ids=top_ids, g_top=g_top, dlogits=dlogits)
-  xt = _row_vec(xt, 'xt', logits, torch.int64)
-  x0 = _row_vec(x0, 'x0', logits, torch.int64)
-  lse = _row_vec(lse, 'lse', logits, torch.float32)
-  entropy = _row_vec(entropy, 'entropy', logits, torch.float32)
+  shape, dev = logits.shape[:-1], lg.get_device()
+  xt = _row_vec(xt, 'xt', shape, dev, torch.int64)
+  x0 = _row_vec(x0, 'x0', shape, dev, torch.int64)
+  lse = _row_vec(lse, 'lse', shape, dev, torch.float32)
+  entropy = _row_vec(entropy, 'entropy', shape, dev, torch.float32)
   if g_logp is not None:
-    g_logp = _row_vec(g_logp, 'g_logp', logits, torch.float32)
+    g_logp = _row_vec(g_logp, 'g_logp', shape, dev, torch.float32)
   if g_entropy is not None:
-    g_entropy = _row_vec(g_entropy, 'g_entropy', logits, torch.float32)
+    g_entropy = _row_vec(g_entropy, 'g_entropy', shape, dev, torch.float32)
   k = 0
   if g_top is not None:
     k = g_top.shape[-1]
-    if top_ids is None or top_ids.shape != g_top.shape or g_top.shape[:-1] != logits.shape[:-1]:
-      raise RuntimeError('g_top: needs top_ids of the same shape, one row per row of logits')
     if k > 64 or (k and k >= V):
       raise RuntimeError(f'g_top: {k} alternatives, at most 64 and less than V={V}')
-    g_top = _dev(g_top, 'g_top', torch.float32).contiguous()
-    top_ids = _dev(top_ids, 'top_ids', torch.int64).contiguous()
-  with torch.cuda.device(lg.device):
+    if top_ids is None:
+      raise RuntimeError('g_top: needs top_ids')
+    g_top = _row_vec(g_top, 'g_top', (*shape, k), dev, torch.float32)
+    top_ids = _row_vec(top_ids, 'top_ids', (*shape, k), dev, torch.int64)
+  with _on_device(lg) as stream:
     if dlogits is None:
-      if logits.dim() == 3:
-        dlogits = alloc_logits(logits.shape[0], logits.shape[1], V, lg.dtype, lg.device)
-      else:
-        dlogits = torch.empty(rows, padded_vocab(V), dtype=lg.dtype, device=lg.device)[:, :V]
-    o, orows, oV, ldo = _rows2d(dlogits, 'dlogits')
+      ld_new = padded_vocab(V)
+      dlogits = torch.empty((*shape, ld_new), dtype=lg.dtype, device=lg.device)
+      if ld_new != V:
+        dlogits = dlogits[..., :V]
+    _same_device(lg, dlogits=dlogits)
+    o, _, _, ldo = _rows2d(dlogits, 'dlogits')
     if o.dtype != lg.dtype or dlogits.shape != logits.shape:
       raise RuntimeError(f'dlogits: expected {tuple(logits.shape)} {lg.dtype}, got {tuple(dlogits.shape)} {o.dtype}')
     call('mdlm_subs_scores_bwd', lg.data_ptr(), ld, _DT[lg.dtype], xt.data_ptr(), x0.data_ptr(),
          lse.data_ptr(), entropy.data_ptr(), _p(g_logp), _p(g_entropy), _p(top_ids) if k else 0,
-         _p(g_top) if k else 0, k, o.data_ptr(), ldo, rows, V, int(mask_index), _stream())
+         _p(g_top) if k else 0, k, o.data_ptr(), ldo, rows, V, int(mask_index), stream)
   return dlogits
 
 
@@ -768,7 +789,7 @@ def orthogonalize(g, steps=5, coeffs=MUON_COEFFS, eps=1e-7, out=None, ws=None):
   `workspace('orthogonalize', n, rows, cols)`, allocated if not given."""
   n, r, c, ld, bs = _matrices(g, 'g', _DT)
   _same_device(g, out=out, ws=ws)
-  with torch.cuda.device(g.device):
+  with _on_device(g) as stream:
     if out is None:
       out = torch.empty(g.shape, dtype=torch.bfloat16, device=g.device)
     if out.shape != g.shape:
@@ -777,7 +798,7 @@ def orthogonalize(g, steps=5, coeffs=MUON_COEFFS, eps=1e-7, out=None, ws=None):
     if g.numel():
       ws = _ortho_ws(ws, n, r, c, g.device)
       call('mdlm_orthogonalize', g.data_ptr(), ld, bs, _DT[g.dtype], out.data_ptr(), ldo, bso, n, r, c,
-           int(steps), float(coeffs[0]), float(coeffs[1]), float(coeffs[2]), float(eps), ws.data_ptr(), _stream())
+           int(steps), float(coeffs[0]), float(coeffs[1]), float(coeffs[2]), float(eps), ws.data_ptr(), stream)
   return out
 
 
@@ -811,10 +832,10 @@ def muon_update(p, g, m, lr, ema=None, w16=None, momentum=0.95, weight_decay=0.0
   if scale is None:
     scale = 0.2 * math.sqrt(max(r, c))
   if p.numel():
-    with torch.cuda.device(p.device):
+    with _on_device(p) as stream:
       ws = _ortho_ws(ws, n, r, c, p.device)
       call('mdlm_muon_update', p.data_ptr(), g.data_ptr(), m.data_ptr(), _p(ema), _p(w16), ld, bs, n, r, c,
            float(lr), float(momentum), float(weight_decay), float(scale), int(steps), float(coeffs[0]),
            float(coeffs[1]), float(coeffs[2]), float(eps), float(ema_one_minus_decay), _p(sumsq),
-           float(max_norm), float(grad_scale), ws.data_ptr(), _stream())
+           float(max_norm), float(grad_scale), ws.data_ptr(), stream)
   return p
