@@ -29,8 +29,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int NS_TILE = 128;
 constexpr int NS_BK = 64;
+constexpr int NS_FEW_TILES = 200;     // of 128 x 128: fewer leave CUs idle, 64 x 64 tiles then
 constexpr int NS_NORM_BLOCKS = 256;   // partial sums of |G|^2 per matrix
 // Powers of two that keep the fp16 words away from the subnormal range: entries
 // of X are at most about 1.2 and about 1/sqrt(s l) on average, D and P are at
@@ -39,13 +39,16 @@ constexpr float NS_SX = 2048.f;
 constexpr float NS_SD = 256.f;
 
 struct NsShape { int s, l, sp, lp; bool tall; };
-static inline NsShape ns_shape(int rows, int cols) {
+static inline NsShape ns_shape(int n, int rows, int cols) {
   NsShape q;
   q.tall = rows > cols;
   q.s = q.tall ? cols : rows;
   q.l = q.tall ? rows : cols;
-  q.sp = (q.s + NS_TILE - 1) / NS_TILE * NS_TILE;
-  q.lp = (q.l + NS_TILE - 1) / NS_TILE * NS_TILE;
+  // whole tiles of the largest that may be used
+  const int64_t t128 = (int64_t)n * ((q.s + 127) / 128) * ((q.l + 127) / 128);
+  const int t = t128 < NS_FEW_TILES ? 64 : 128;
+  q.sp = (q.s + t - 1) / t * t;
+  q.lp = (q.l + t - 1) / t * t;
   return q;
 }
 
@@ -53,7 +56,6 @@ static inline NsShape ns_shape(int rows, int cols) {
 struct NsWs {
   double* norm;      // n x NS_NORM_BLOCKS partial sums of squares
   float* diag;       // n x sp
-  float* o;          // n x sp x lp, the result of the last step
   f16 *h[2], *lo;    // n x sp x lp
   f16 *d, *p;        // n x sp x sp
 };
@@ -64,7 +66,6 @@ static inline int64_t ns_layout(const NsShape& q, int n, char* base, NsWs* w) {
   NsWs t;
   t.norm = (double*)take((int64_t)n * NS_NORM_BLOCKS * 8);
   t.diag = (float*)take((int64_t)n * q.sp * 4);
-  t.o = (float*)take(x * 4);
   t.h[0] = (f16*)take(x * 2);
   t.h[1] = (f16*)take(x * 2);
   t.lo = (f16*)take(x * 2);
@@ -160,229 +161,362 @@ __global__ __launch_bounds__(256) void ns_ingest_kernel(NsSrc a, const double* _
   }
 }
 
-enum { NS_GRAM = 0, NS_SQUARE = 1, NS_APPLY = 2 };
-
-struct NsGemm {
-  const f16* A; int64_t lda, bsa;    // M x K, K contiguous
-  const f16* B; int64_t ldb, bsb;    // N x K, K contiguous (APPLY: K x N, N contiguous)
-  int K, tiles_m, tiles_n, n;
-  f16* out; int64_t ldo, bso;        // D, P or the next X's high words
-  f16* lo;                           // APPLY: low words of X, in place
-  float* o;                          // APPLY, last step: fp32 result (null: not the last)
-  float* diag; int sp;               // rounding of D's diagonal
-  float shift, c, mu;                // b/2c; c; see the head of this file
-};
-
-#define NS_GLDS16(gptr, lptr) \
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(gptr), \
-                                   (__attribute__((address_space(3))) void*)(lptr), 16, 0, 0)
-
-// 128 x 128 tile, 4 waves of 64 x 64, 64-deep slabs double-buffered in LDS by LDS-DMA.
-// LDS rows of a K-contiguous operand hold 64 values (128 bytes); the 16-byte chunk
-// index is XORed with row & 7 on the source address and on the fragment reads.  The
-// N-contiguous operand of APPLY keeps its rows (128 columns, 256 bytes) and is
-// read through the transposing LDS read (four rows x 16 columns per 16 lanes);
-// its 32-byte blocks are XORed with (row & 3) | (row >> 3 & 1) << 2.
-template <int MODE>
-__global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsGemm g) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int OP = NS_TILE * NS_BK * 2, STAGE = 2 * OP;   // 16 KiB per operand
-  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wr = wid >> 1, wc = wid & 1;
-  const int per_mat = g.tiles_m * g.tiles_n, total = per_mat * g.n;
-  // each XCD (workgroup id & 7) gets a contiguous range of tiles
-  const int per_xcd = (total + 7) >> 3;
-  const int idx = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per_xcd || idx >= total) return;
-  const int b = idx / per_mat, rest = idx - b * per_mat;
-  const int tm = rest / g.tiles_n, tn = rest - tm * g.tiles_n;
-  const f16* A = g.A + b * g.bsa + (int64_t)tm * NS_TILE * g.lda;
-  const f16* B = g.B + b * g.bsb + (MODE == NS_APPLY ? (int64_t)tn * NS_TILE : (int64_t)tn * NS_TILE * g.ldb);
-
-  const int arow = lane >> 3, achunk = ((lane & 7) ^ arow) * 8;
-  const f16* a_src = A + (int64_t)(wid * 8 + arow) * g.lda + achunk;
-  const f16* b_src;
-  if constexpr (MODE == NS_APPLY) {
-    const int row = wid * 4 + (lane >> 4), pch = lane & 15;
-    const int fx = (row & 3) | (((row >> 3) & 1) << 2);      // + 16 rows: unchanged
-    b_src = B + (int64_t)row * g.ldb + (((pch >> 1) ^ fx) * 2 + (pch & 1)) * 8;
-  } else {
-    b_src = B + (int64_t)(wid * 8 + arow) * g.ldb + achunk;
-  }
-  auto stage = [&](int buf, int k0) {
-    char* const sb = smem + buf * STAGE;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      NS_GLDS16(a_src + (int64_t)(i * 32) * g.lda + k0, sb + (i * 4 + wid) * 1024);
-      if constexpr (MODE == NS_APPLY)
-        NS_GLDS16(b_src + (int64_t)(k0 + i * 16) * g.ldb, sb + OP + (i * 4 + wid) * 1024);
-      else
-        NS_GLDS16(b_src + (int64_t)(i * 32) * g.ldb + k0, sb + OP + (i * 4 + wid) * 1024);
-    }
-  };
-  const int fr = lane & 15, fq = lane >> 4;
-  int foff[2];
-#pragma unroll
-  for (int ks = 0; ks < 2; ++ks) foff[ks] = fr * 128 + (((ks * 4 + fq) ^ (lane & 7)) * 16);
-  const int a_base = wr * 64 * 128, b_base = OP + wc * 64 * 128;
-  unsigned tr_off[4];
-  const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
-  if constexpr (MODE == NS_APPLY) {
-    const int q = fr >> 2, p = lane & 3, fx = q | ((fq & 1) << 2);
-#pragma unroll
-    for (int n = 0; n < 4; ++n) tr_off[n] = lds0 + OP + (8 * fq + q) * 256 + (((wc * 4 + n) ^ fx) * 32) + p * 8;
-  }
-  f32x4 acc[4][4];
-#pragma unroll
-  for (int m = 0; m < 4; ++m)
-#pragma unroll
-    for (int n = 0; n < 4; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-
-  stage(0, 0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  const int KT = g.K / NS_BK;
-  for (int kt = 0; kt < KT; ++kt) {
-    const int buf = kt & 1;
-    if (kt + 1 < KT) stage(buf ^ 1, (kt + 1) * NS_BK);
-    const char* sb = smem + buf * STAGE;
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      f16x8 af[4], bf[4];
-#pragma unroll
-      for (int m = 0; m < 4; ++m) af[m] = *reinterpret_cast<const f16x8*>(sb + a_base + m * 2048 + foff[ks]);
-      if constexpr (MODE == NS_APPLY) {
-        // the reads and their wait in one block: the compiler does not count them
-        uint2 t[8];
-        const unsigned o = buf * STAGE + ks * 32 * 256;
-        const unsigned a0 = tr_off[0] + o, a1 = tr_off[1] + o, a2 = tr_off[2] + o, a3 = tr_off[3] + o;
-        asm volatile(
-          "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:1024\n\t"
-          "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:1024\n\t"
-          "ds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:1024\n\t"
-          "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:1024\n\t"
-          "s_waitcnt lgkmcnt(0)"
-          : "=&v"(t[0]), "=&v"(t[1]), "=&v"(t[2]), "=&v"(t[3]), "=&v"(t[4]), "=&v"(t[5]), "=&v"(t[6]), "=&v"(t[7])
-          : "v"(a0), "v"(a1), "v"(a2), "v"(a3) : "memory");
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-          bf[n] = __builtin_bit_cast(f16x8, make_uint4(t[2 * n].x, t[2 * n].y, t[2 * n + 1].x, t[2 * n + 1].y));
-      } else {
-#pragma unroll
-        for (int n = 0; n < 4; ++n) bf[n] = *reinterpret_cast<const f16x8*>(sb + b_base + n * 2048 + foff[ks]);
-      }
-      // swapped operands: a lane holds four consecutive columns of one output row
-#pragma unroll
-      for (int m = 0; m < 4; ++m)
-#pragma unroll
-        for (int n = 0; n < 4; ++n)
-          acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf[n], af[m], acc[m][n], 0, 0, 0);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the next slab has landed
-    __syncthreads();
-  }
-
-#pragma unroll
-  for (int m = 0; m < 4; ++m) {
-    const int i = tm * NS_TILE + wr * 64 + m * 16 + fr;
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-      const int j = tn * NS_TILE + wc * 64 + n * 16 + fq * 4;
-      const int64_t at = b * g.bso + (int64_t)i * g.ldo + j;
-      f16x4 hv;
-      if constexpr (MODE == NS_GRAM) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = acc[m][n][e] * (NS_SD / (NS_SX * NS_SX));
-          if (i == j + e) v += g.shift * NS_SD;
-          hv[e] = (f16)v;
-          if (i == j + e) g.diag[b * g.sp + i] = v - (float)hv[e];
-        }
-        *reinterpret_cast<f16x4*>(g.out + at) = hv;
-      } else if constexpr (MODE == NS_SQUARE) {
-        const f16x4 dv = *reinterpret_cast<const f16x4*>(g.A + at);      // D at the output's place
-        const float di = g.diag[b * g.sp + i];
-        const f32x4 dj = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float v = (acc[m][n][e] + (di + dj[e]) * (float)dv[e]) * (g.c / NS_SD);
-          if (i == j + e) v += g.mu * NS_SD;      // (a - b^2/4c) - mu
-          hv[e] = (f16)v;
-        }
-        *reinterpret_cast<f16x4*>(g.out + at) = hv;
-      } else {
-        const f16x4 xh = *reinterpret_cast<const f16x4*>(g.B + at), xl = *reinterpret_cast<const f16x4*>(g.lo + at);
-        f32x4 v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[e] = g.mu * ((float)xh[e] + (float)xl[e]) + acc[m][n][e] * (1.f / NS_SD);
-        if (g.o) {
-          *reinterpret_cast<f32x4*>(g.o + at) = v * (1.f / NS_SX);
-        } else {
-          f16x4 lv;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { f16 hh, ll; split_f16(v[e], hh, ll); hv[e] = hh; lv[e] = ll; }
-          *reinterpret_cast<f16x4*>(g.out + at) = hv;
-          *reinterpret_cast<f16x4*>(g.lo + at) = lv;
-        }
-      }
-    }
-  }
-}
-
 // The result in the caller's layout, and what is done with it there.
 struct NsOut {
   bf16_t* out;                           // the orthogonalised matrix, or
   float* p; float* ema; bf16_t* w16;     // weights, moving average, bf16 copy
   int64_t ld, bs;
+  int rows, cols;
   float step, decay, ema_omd;            // lr * scale; 1 - lr * weight_decay
+  int vec;                               // rows start 16-byte aligned
 };
-__device__ __forceinline__ void ns_store(const NsOut& w, int64_t at, float o) {
+__device__ __forceinline__ void ns_store1(const NsOut& w, int64_t at, float o) {
   if (w.out) { w.out[at] = f32_to_bf16(o); return; }
   const float p = w.p[at] * w.decay - w.step * o;
   w.p[at] = p;
   if (w.ema) { const float e = w.ema[at]; w.ema[at] = e - w.ema_omd * (e - p); }
   if (w.w16) w.w16[at] = f32_to_bf16(p);
 }
-__global__ __launch_bounds__(256) void ns_out_kernel(NsOut w, const float* __restrict__ o, int rows, int cols, int sp,
-                                                     int lp, int tall) {
-  __shared__ float tile[32][33];
-  const int b = blockIdx.z, tid = threadIdx.x, tx = tid & 31, ty = tid >> 5;
-  const int i0 = blockIdx.y * 32, j0 = blockIdx.x * 32;   // of X
-  for (int k = ty; k < 32; k += 8) tile[k][tx] = o[((int64_t)b * sp + i0 + k) * lp + j0 + tx];
-  __syncthreads();
-  for (int k = ty; k < 32; k += 8) {
-    const int r = tall ? j0 + k : i0 + k, c = tall ? i0 + tx : j0 + tx;
-    if (r < rows && c < cols) ns_store(w, b * w.bs + r * w.ld + c, tall ? tile[tx][k] : tile[k][tx]);
+// eight columns of row r, from column c (a multiple of 8) on
+__device__ __forceinline__ void ns_store8(const NsOut& w, int b, int r, int c, const float (&v)[8]) {
+  if (r >= w.rows) return;
+  const int64_t at = b * w.bs + r * w.ld + c;
+  if (!w.vec || c + 8 > w.cols) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < w.cols) ns_store1(w, at + e, v[e]);
+    return;
   }
+  float p[8];
+  if (w.out) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = v[e];
+  } else {
+    f32x4 q[2], m[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) q[h] = *reinterpret_cast<const f32x4*>(w.p + at + 4 * h);
+    if (w.ema) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) m[h] = *reinterpret_cast<const f32x4*>(w.ema + at + 4 * h);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e >> 2][e & 3] = p[e] = q[e >> 2][e & 3] * w.decay - w.step * v[e];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) *reinterpret_cast<f32x4*>(w.p + at + 4 * h) = q[h];
+    if (w.ema) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<f32x4*>(w.ema + at + 4 * h) = m[h] - w.ema_omd * (m[h] - q[h]);
+    }
+    if (!w.w16) return;
+  }
+  *reinterpret_cast<uint4*>((w.out ? w.out : w.w16) + at) =
+    make_uint4(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(p[4], p[5]), pack_bf16x2(p[6], p[7]));
 }
 
-static int ns_gemm(int mode, NsGemm g, hipStream_t st) {
-  constexpr int LDS = 4 * NS_TILE * NS_BK * 2;
-  static bool done[3][MAX_DEVICES] = {};
-  const int64_t total = (int64_t)g.tiles_m * g.tiles_n * g.n;
-  if (total >= (1ll << 28)) { set_error("orthogonalize: too many tiles"); return -1; }
-  const unsigned grid = (unsigned)((total + 7) / 8 * 8);
-  int rc;
-  if (mode == NS_GRAM) {
-    if ((rc = ensure_dynamic_lds(&ns_gemm_kernel<NS_GRAM>, LDS, done[0], "orthogonalize"))) return rc;
-    ns_gemm_kernel<NS_GRAM><<<grid, 256, LDS, st>>>(g);
-  } else if (mode == NS_SQUARE) {
-    if ((rc = ensure_dynamic_lds(&ns_gemm_kernel<NS_SQUARE>, LDS, done[1], "orthogonalize"))) return rc;
-    ns_gemm_kernel<NS_SQUARE><<<grid, 256, LDS, st>>>(g);
-  } else {
-    if ((rc = ensure_dynamic_lds(&ns_gemm_kernel<NS_APPLY>, LDS, done[2], "orthogonalize"))) return rc;
-    ns_gemm_kernel<NS_APPLY><<<grid, 256, LDS, st>>>(g);
+enum { NS_GRAM = 0, NS_SQUARE = 1, NS_APPLY = 2 };
+
+struct NsGemm {
+  const f16* A; int64_t lda, bsa;    // M x K, K contiguous
+  const f16* B; int64_t ldb, bsb;    // N x K, K contiguous (APPLY: K x N, N contiguous)
+  int K, M, N, n;                    // of one matrix, whole tiles; n matrices
+  f16* out; int64_t ldo, bso;        // D, P or the next X's high words
+  f16* lo;                           // APPLY: low words of X, in place
+  float* diag; int sp;               // rounding of D's diagonal
+  float shift, c, mu;                // see the head of this file
+  int last, tall;                    // APPLY: the result goes to dst
+  NsOut dst;
+};
+
+#define NS_GLDS16(gptr, lptr) \
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(gptr), \
+                                   (__attribute__((address_space(3))) void*)(lptr), 16, 0, 0)
+
+// All but the last `slabs` slabs in flight have landed, for this wave and then for
+// the workgroup; this wave's own LDS reads are done too.
+template <int L>
+__device__ __forceinline__ void slab_wait(int slabs) {
+  if (slabs >= 3) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(3 * L) : "memory");
+  else if (slabs == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * L) : "memory");
+  else if (slabs == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(L) : "memory");
+  else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// T x T tile, 4 waves of T/2 x T/2, slabs of 64 in an LDS ring of NST by LDS-DMA.
+// LDS rows of a K-contiguous operand hold 64 values (128 bytes); the 16-byte chunk
+// index is XORed with row & 7 on the source address and on the fragment reads.  The
+// N-contiguous operand of APPLY keeps its rows (T columns) and is read through the
+// transposing LDS read (four rows x 16 columns per 16 lanes); its 32-byte blocks
+// are XORed so that the eight rows that half a wave reads fall into different banks.
+template <int MODE, int T, int NST>
+struct NsTile {
+  static constexpr int OP = T * NS_BK * 2, STAGE = 2 * OP;
+  static constexpr int WT = T / 2, F = WT / 16;         // wave tile, fragments per side
+  static constexpr int L = T / 32;                      // LDS-DMA instructions per operand, wave and slab
+  static constexpr int PITCH = T + 4;                   // floats per row of the epilogue's tile
+  static constexpr int EPI = T * PITCH * 4;
+  static constexpr int LDS = NST * STAGE > EPI ? NST * STAGE : EPI;
+  static __device__ __forceinline__ int block_xor(int row) {
+    return T == 128 ? (row & 3) | (((row >> 3) & 1) << 2) : ((row >> 1) & 1) | (((row >> 3) & 1) << 1);
   }
+
+  static __device__ __forceinline__ void run(const NsGemm& g, int b, int tm, int tn, char* smem) {
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wid >> 1, wc = wid & 1, fr = lane & 15, fq = lane >> 4;
+    const f16* A = g.A + b * g.bsa + (int64_t)tm * T * g.lda;
+    const f16* B = g.B + b * g.bsb + (MODE == NS_APPLY ? (int64_t)tn * T : (int64_t)tn * T * g.ldb);
+    const int arow = lane >> 3, achunk = ((lane & 7) ^ arow) * 8;
+    const f16* a_src = A + (int64_t)(wid * 8 + arow) * g.lda + achunk;
+    // APPLY: a wave instruction covers 1024 / (2 T) rows of the slab
+    constexpr int RI = 512 / T, CL = T / 8;
+    const f16* b_src;
+    if constexpr (MODE == NS_APPLY) {
+      // this wave's instructions are 4 RI rows apart: the XOR term is the same for all
+      const int row = wid * RI + lane / CL, pch = lane % CL;
+      b_src = B + (int64_t)row * g.ldb + (((pch >> 1) ^ block_xor(row)) * 2 + (pch & 1)) * 8;
+    } else {
+      b_src = B + (int64_t)(wid * 8 + arow) * g.ldb + achunk;
+    }
+    auto stage = [&](int st, int k0) {
+      char* const sb = smem + st * STAGE;
+#pragma unroll
+      for (int i = 0; i < L; ++i) {
+        NS_GLDS16(a_src + (int64_t)(i * 32) * g.lda + k0, sb + (i * 4 + wid) * 1024);
+        if constexpr (MODE == NS_APPLY)
+          NS_GLDS16(b_src + (int64_t)(k0 + i * 4 * RI) * g.ldb, sb + OP + (i * 4 + wid) * 1024);
+        else
+          NS_GLDS16(b_src + (int64_t)(i * 32) * g.ldb + k0, sb + OP + (i * 4 + wid) * 1024);
+      }
+    };
+    int foff[2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) foff[ks] = fr * 128 + (((ks * 4 + fq) ^ (lane & 7)) * 16);
+    const int a_base = wr * WT * 128, b_base = OP + wc * WT * 128;
+    unsigned tr[F];
+    if constexpr (MODE == NS_APPLY) {
+      const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
+      const int row = 8 * fq + (fr >> 2);       // + 4, + 32: the same XOR term
+#pragma unroll
+      for (int n = 0; n < F; ++n)
+        tr[n] = lds0 + OP + row * (2 * T) + (((wc * F + n) ^ block_xor(row)) * 32) + (lane & 3) * 8;
+    }
+    f32x4 acc[F][F];
+#pragma unroll
+    for (int m = 0; m < F; ++m)
+#pragma unroll
+      for (int n = 0; n < F; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+    const int KT = g.K / NS_BK;
+#pragma unroll
+    for (int i = 0; i < NST - 1; ++i)
+      if (i < KT) stage(i, i * NS_BK);
+    int st = 0, st_in = NST - 1;      // ring slots read and filled next
+    for (int kt = 0; kt < KT; ++kt) {
+      const int behind = KT - 1 - kt;
+      slab_wait<2 * L>(behind < NST - 2 ? behind : NST - 2);
+      if (kt + NST - 1 < KT) stage(st_in, (kt + NST - 1) * NS_BK);
+      const char* sb = smem + st * STAGE;
+      f16x8 af[2][F], bf[2][F];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int m = 0; m < F; ++m) af[ks][m] = *reinterpret_cast<const f16x8*>(sb + a_base + m * 2048 + foff[ks]);
+      if constexpr (MODE == NS_APPLY) {
+        // the reads and their wait in one block: the compiler does not count them
+        uint2 t[2][F][2];
+        const unsigned o = st * STAGE;
+        if constexpr (F == 4) {
+          const unsigned a0 = tr[0] + o, a1 = tr[1] + o, a2 = tr[2] + o, a3 = tr[3] + o;
+          asm volatile(
+            "ds_read_b64_tr_b16 %0, %16\n\tds_read_b64_tr_b16 %1, %16 offset:1024\n\t"
+            "ds_read_b64_tr_b16 %2, %17\n\tds_read_b64_tr_b16 %3, %17 offset:1024\n\t"
+            "ds_read_b64_tr_b16 %4, %18\n\tds_read_b64_tr_b16 %5, %18 offset:1024\n\t"
+            "ds_read_b64_tr_b16 %6, %19\n\tds_read_b64_tr_b16 %7, %19 offset:1024\n\t"
+            "ds_read_b64_tr_b16 %8, %16 offset:8192\n\tds_read_b64_tr_b16 %9, %16 offset:9216\n\t"
+            "ds_read_b64_tr_b16 %10, %17 offset:8192\n\tds_read_b64_tr_b16 %11, %17 offset:9216\n\t"
+            "ds_read_b64_tr_b16 %12, %18 offset:8192\n\tds_read_b64_tr_b16 %13, %18 offset:9216\n\t"
+            "ds_read_b64_tr_b16 %14, %19 offset:8192\n\tds_read_b64_tr_b16 %15, %19 offset:9216\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(t[0][0][0]), "=&v"(t[0][0][1]), "=&v"(t[0][1][0]), "=&v"(t[0][1][1]), "=&v"(t[0][2][0]),
+              "=&v"(t[0][2][1]), "=&v"(t[0][3][0]), "=&v"(t[0][3][1]), "=&v"(t[1][0][0]), "=&v"(t[1][0][1]),
+              "=&v"(t[1][1][0]), "=&v"(t[1][1][1]), "=&v"(t[1][2][0]), "=&v"(t[1][2][1]), "=&v"(t[1][3][0]),
+              "=&v"(t[1][3][1])
+            : "v"(a0), "v"(a1), "v"(a2), "v"(a3) : "memory");
+        } else {
+          const unsigned a0 = tr[0] + o, a1 = tr[1] + o;
+          asm volatile(
+            "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:512\n\t"
+            "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:512\n\t"
+            "ds_read_b64_tr_b16 %4, %8 offset:4096\n\tds_read_b64_tr_b16 %5, %8 offset:4608\n\t"
+            "ds_read_b64_tr_b16 %6, %9 offset:4096\n\tds_read_b64_tr_b16 %7, %9 offset:4608\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(t[0][0][0]), "=&v"(t[0][0][1]), "=&v"(t[0][1][0]), "=&v"(t[0][1][1]), "=&v"(t[1][0][0]),
+              "=&v"(t[1][0][1]), "=&v"(t[1][1][0]), "=&v"(t[1][1][1])
+            : "v"(a0), "v"(a1) : "memory");
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int n = 0; n < F; ++n)
+            bf[ks][n] = __builtin_bit_cast(f16x8, make_uint4(t[ks][n][0].x, t[ks][n][0].y, t[ks][n][1].x, t[ks][n][1].y));
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int n = 0; n < F; ++n) bf[ks][n] = *reinterpret_cast<const f16x8*>(sb + b_base + n * 2048 + foff[ks]);
+      }
+      // swapped operands: a lane holds four consecutive columns of one output row
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int m = 0; m < F; ++m)
+#pragma unroll
+          for (int n = 0; n < F; ++n)
+            acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf[ks][n], af[ks][m], acc[m][n], 0, 0, 0);
+      st = st + 1 == NST ? 0 : st + 1;
+      st_in = st_in + 1 == NST ? 0 : st_in + 1;
+    }
+    // ---- epilogue: the sums through LDS, so that global rows are read and written whole
+    __syncthreads();
+    float* const tile = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int m = 0; m < F; ++m)
+#pragma unroll
+      for (int n = 0; n < F; ++n)
+        *reinterpret_cast<f32x4*>(tile + (wr * WT + m * 16 + fr) * PITCH + wc * WT + n * 16 + fq * 4) = acc[m][n];
+    __syncthreads();
+    const int i0 = tm * T, j0 = tn * T;
+    // eight outputs at (i, j..j+7)
+    auto put = [&](int i, int j, const float (&v)[8]) {
+      const int64_t at = b * g.bso + (int64_t)i * g.ldo + j;
+      f16x8 hv;
+      if constexpr (MODE == NS_GRAM) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float x = v[e] * (NS_SD / (NS_SX * NS_SX));
+          if (i == j + e) x += g.shift * NS_SD;
+          hv[e] = (f16)x;
+          if (i == j + e) g.diag[b * g.sp + i] = x - (float)hv[e];
+        }
+        *reinterpret_cast<f16x8*>(g.out + at) = hv;
+      } else {   // NS_SQUARE
+        const f16x8 dv = *reinterpret_cast<const f16x8*>(g.A + at);
+        const float di = g.diag[b * g.sp + i];
+        const f32x4 d0 = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j);
+        const f32x4 d1 = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j + 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float x = (v[e] + (di + (e < 4 ? d0[e & 3] : d1[e & 3])) * (float)dv[e]) * (g.c / NS_SD);
+          if (i == j + e) x += g.mu * NS_SD;      // (a - b^2/4c) - mu
+          hv[e] = (f16)x;
+        }
+        *reinterpret_cast<f16x8*>(g.out + at) = hv;
+      }
+    };
+    constexpr int CH = T / 8, RP = 256 / CH;            // chunks of 8 per row, rows per pass
+    const int pr = tid / CH, pc = (tid % CH) * 8;
+#pragma unroll
+    for (int r = 0; r < T; r += RP) {
+      const int i = r + pr;
+      const f32x4 lo4 = *reinterpret_cast<const f32x4*>(tile + i * PITCH + pc);
+      const f32x4 hi4 = *reinterpret_cast<const f32x4*>(tile + i * PITCH + pc + 4);
+      const float v[8] = {lo4[0], lo4[1], lo4[2], lo4[3], hi4[0], hi4[1], hi4[2], hi4[3]};
+      if constexpr (MODE != NS_APPLY) {
+        put(i0 + i, j0 + pc, v);
+      } else {
+        const int64_t at = b * g.bso + (int64_t)(i0 + i) * g.ldo + j0 + pc;
+        const f16x8 xh = *reinterpret_cast<const f16x8*>(g.B + at), xl = *reinterpret_cast<const f16x8*>(g.lo + at);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = g.mu * ((float)xh[e] + (float)xl[e]) + v[e] * (1.f / NS_SD);
+        if (!g.last) {
+          f16x8 hv, lv;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) { f16 hh, ll; split_f16(x[e], hh, ll); hv[e] = hh; lv[e] = ll; }
+          *reinterpret_cast<f16x8*>(g.out + at) = hv;
+          *reinterpret_cast<f16x8*>(g.lo + at) = lv;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] *= 1.f / NS_SX;
+          if (!g.tall) {
+            ns_store8(g.dst, b, i0 + i, j0 + pc, x);
+          } else {
+            *reinterpret_cast<f32x4*>(tile + i * PITCH + pc) = (f32x4){x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<f32x4*>(tile + i * PITCH + pc + 4) = (f32x4){x[4], x[5], x[6], x[7]};
+          }
+        }
+      }
+    }
+    // the other side of a symmetric product, or a tall matrix's own orientation:
+    // 16 columns x 4 chunks of 8 rows per wave and pass
+    const bool turn = MODE == NS_APPLY ? g.last && g.tall : tm != tn;
+    if (turn) {
+      if constexpr (MODE == NS_APPLY) __syncthreads();
+#pragma unroll 4
+      for (int q = wid; q < (T / 16) * (T / 32); q += 4) {
+        const int j = (q % (T / 16)) * 16 + fr, i = (q / (T / 16)) * 32 + fq * 8;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = tile[(i + e) * PITCH + j];
+        if constexpr (MODE == NS_APPLY) ns_store8(g.dst, b, j0 + j, i0 + i, v);
+        else put(j0 + j, i0 + i, v);
+      }
+    }
+  }
+};
+
+// Tiles of GRAM and SQUARE: the lower triangle of a symmetric result (t = 0: (0,0),
+// then (1,0), (1,1), ..).
+__device__ __forceinline__ void triangle(int t, int& tm, int& tn) {
+  tm = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+  while (tm * (tm + 1) / 2 > t) --tm;
+  while ((tm + 1) * (tm + 2) / 2 <= t) ++tm;
+  tn = t - tm * (tm + 1) / 2;
+}
+
+template <int MODE, int T, int NST>
+__global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsGemm g) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tiles_m = g.M / T, tiles_n = g.N / T;
+  const int per_mat = MODE == NS_APPLY ? tiles_m * tiles_n : tiles_m * (tiles_m + 1) / 2, total = per_mat * g.n;
+  // each XCD (workgroup id & 7) gets a contiguous range of tiles
+  const int per_xcd = (total + 7) >> 3;
+  const int idx = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per_xcd || idx >= total) return;
+  const int b = idx / per_mat, t = idx - b * per_mat;
+  int tm, tn;
+  if (MODE == NS_APPLY) { tn = t / tiles_m; tm = t - tn * tiles_m; }     // X's columns are read once per XCD
+  else triangle(t, tm, tn);
+  NsTile<MODE, T, NST>::run(g, b, tm, tn, smem);
+}
+
+template <int MODE, int T, int NST>
+static int ns_launch(const NsGemm& g, hipStream_t st) {
+  constexpr int LDS = NsTile<MODE, T, NST>::LDS;
+  static bool done[MAX_DEVICES] = {};
+  if (int rc = ensure_dynamic_lds(&ns_gemm_kernel<MODE, T, NST>, LDS, done, "orthogonalize")) return rc;
+  const int64_t tm = g.M / T, tn = g.N / T, total = (MODE == NS_APPLY ? tm * tn : tm * (tm + 1) / 2) * g.n;
+  if (total >= (1ll << 28)) { set_error("orthogonalize: too many tiles"); return -1; }
+  ns_gemm_kernel<MODE, T, NST><<<(unsigned)((total + 7) / 8 * 8), 256, LDS, st>>>(g);
   MDLM_LAUNCH_CHECK();
   return 0;
 }
+template <int MODE>
+static int ns_gemm(const NsGemm& g, hipStream_t st) {
+  const int64_t tm = g.M / 128, tn = g.N / 128;
+  const int64_t tiles = (MODE == NS_APPLY ? tm * tn : tm * (tm + 1) / 2) * g.n;
+  if (g.M % 128 || g.N % 128 || tiles < NS_FEW_TILES) return ns_launch<MODE, 64, 4>(g, st);
+  return ns_launch<MODE, 128, 2>(g, st);
+}
 
-static int ns_run(const NsSrc& src, const NsOut& dst, int n, int rows, int cols, int steps, double a, double b,
-                  double c, double eps, void* ws, hipStream_t st) {
-  const NsShape q = ns_shape(rows, cols);
+static int ns_run(const NsSrc& src, NsOut dst, int n, int rows, int cols, int steps, double a, double b, double c,
+                  double eps, void* ws, hipStream_t st) {
+  const NsShape q = ns_shape(n, rows, cols);
   NsWs w;
   ns_layout(q, n, (char*)ws, &w);
+  dst.rows = rows; dst.cols = cols;
+  dst.vec = (dst.ld | dst.bs) % 8 == 0 &&
+            (((uintptr_t)dst.out | (uintptr_t)dst.p | (uintptr_t)dst.ema | (uintptr_t)dst.w16) & 15) == 0;
   ns_norm_kernel<<<dim3(NS_NORM_BLOCKS, n), 256, 0, st>>>(src, w.norm, rows, cols);
   MDLM_LAUNCH_CHECK();
   const dim3 grid32(q.lp / 32, q.sp / 32, n);
@@ -395,19 +529,17 @@ static int ns_run(const NsSrc& src, const NsOut& dst, int n, int rows, int cols,
     NsGemm g = {};
     g.n = n; g.sp = q.sp; g.diag = w.diag;
     g.A = x; g.lda = q.lp; g.bsa = bx; g.B = x; g.ldb = q.lp; g.bsb = bx; g.K = q.lp;
-    g.tiles_m = g.tiles_n = q.sp / NS_TILE;
+    g.M = g.N = q.sp;
     g.out = w.d; g.ldo = q.sp; g.bso = bd; g.shift = (float)(b / (2 * c));
-    if (int rc = ns_gemm(NS_GRAM, g, st)) return rc;
+    if (int rc = ns_gemm<NS_GRAM>(g, st)) return rc;
     g.A = w.d; g.lda = q.sp; g.bsa = bd; g.B = w.d; g.ldb = q.sp; g.bsb = bd; g.K = q.sp;
     g.out = w.p; g.c = (float)c; g.mu = (float)(a - b * b / (4 * c) - mu);
-    if (int rc = ns_gemm(NS_SQUARE, g, st)) return rc;
-    g.A = w.p; g.B = x; g.ldb = q.lp; g.bsb = bx; g.tiles_n = q.lp / NS_TILE;
+    if (int rc = ns_gemm<NS_SQUARE>(g, st)) return rc;
+    g.A = w.p; g.B = x; g.ldb = q.lp; g.bsb = bx; g.N = q.lp;
     g.out = xn; g.ldo = q.lp; g.bso = bx; g.lo = w.lo; g.mu = (float)mu;
-    g.o = it + 1 == steps ? w.o : nullptr;
-    if (int rc = ns_gemm(NS_APPLY, g, st)) return rc;
+    g.last = it + 1 == steps; g.tall = q.tall; g.dst = dst;
+    if (int rc = ns_gemm<NS_APPLY>(g, st)) return rc;
   }
-  ns_out_kernel<<<grid32, 256, 0, st>>>(dst, w.o, rows, cols, q.sp, q.lp, q.tall);
-  MDLM_LAUNCH_CHECK();
   return 0;
 }
 
@@ -432,7 +564,7 @@ using namespace mdlm;
 
 extern "C" int64_t mdlm_orthogonalize_workspace_bytes(int n, int rows, int cols) {
   if (n <= 0 || rows <= 0 || cols <= 0 || n >= 65536 || rows > (1 << 17) || cols > (1 << 17)) return -1;
-  return ns_layout(ns_shape(rows, cols), n, nullptr, nullptr);
+  return ns_layout(ns_shape(n, rows, cols), n, nullptr, nullptr);
 }
 
 extern "C" int mdlm_orthogonalize(const void* g, int64_t ldg, int64_t g_stride, int dtype, void* out_bf16, int64_t ldo,
