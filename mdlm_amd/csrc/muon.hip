@@ -17,8 +17,8 @@
 // 4e-4 .. 1e-3 off (2-norm, relative), less than rounding it to bf16 costs
 // (1.7e-3); plain bf16 operands are 1e-2 .. 3e-2 off.
 //
-// Every matrix is padded with zeros to whole tiles in the workspace, so the
-// products have no edges; padding stays zero through every step.
+// Every matrix is padded with zeros to whole slabs of 64 in the workspace; padding
+// stays zero through every step.
 #include "common.h"
 #include <math.h>
 
@@ -30,7 +30,6 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NS_BK = 64;
-constexpr int NS_FEW_TILES = 200;     // of 128 x 128: fewer leave CUs idle, 64 x 64 tiles then
 constexpr int NS_NORM_BLOCKS = 256;   // partial sums of |G|^2 per matrix
 // Powers of two that keep the fp16 words away from the subnormal range: entries
 // of X are at most about 1.2 and about 1/sqrt(s l) on average, D and P are at
@@ -39,14 +38,12 @@ constexpr float NS_SX = 2048.f;
 constexpr float NS_SD = 256.f;
 
 struct NsShape { int s, l, sp, lp; bool tall; };
-static inline NsShape ns_shape(int n, int rows, int cols) {
+static inline NsShape ns_shape(int rows, int cols) {
   NsShape q;
   q.tall = rows > cols;
   q.s = q.tall ? cols : rows;
   q.l = q.tall ? rows : cols;
-  // whole tiles of the largest that may be used
-  const int64_t t128 = (int64_t)n * ((q.s + 127) / 128) * ((q.l + 127) / 128);
-  const int t = t128 < NS_FEW_TILES ? 64 : 128;
+  const int t = 64;      // slabs of the products
   q.sp = (q.s + t - 1) / t * t;
   q.lp = (q.l + t - 1) / t * t;
   return q;
@@ -234,232 +231,309 @@ struct NsGemm {
 
 // All but the last `slabs` slabs in flight have landed, for this wave and then for
 // the workgroup; this wave's own LDS reads are done too.
-template <int L>
+template <int L, int MAX>
 __device__ __forceinline__ void slab_wait(int slabs) {
-  if (slabs >= 3) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(3 * L) : "memory");
-  else if (slabs == 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * L) : "memory");
-  else if (slabs == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(L) : "memory");
-  else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  if constexpr (MAX > 0) {
+    if (slabs < MAX) { slab_wait<L, MAX - 1>(slabs); return; }
+  }
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(MAX * L) : "memory");
 }
 
-// T x T tile, 4 waves of T/2 x T/2, slabs of 64 in an LDS ring of NST by LDS-DMA.
+// T x T tile of WM x WN waves, slabs of 64 in an LDS ring of NST by LDS-DMA.
 // LDS rows of a K-contiguous operand hold 64 values (128 bytes); the 16-byte chunk
 // index is XORed with row & 7 on the source address and on the fragment reads.  The
 // N-contiguous operand of APPLY keeps its rows (T columns) and is read through the
 // transposing LDS read (four rows x 16 columns per 16 lanes); its 32-byte blocks
 // are XORed so that the eight rows that half a wave reads fall into different banks.
-template <int MODE, int T, int NST>
+// Tiles may reach past M and N: rows and columns are clamped on load, not stored.
+template <int MODE, int T, int WM, int WN, int NST>
 struct NsTile {
-  static constexpr int OP = T * NS_BK * 2, STAGE = 2 * OP;
-  static constexpr int WT = T / 2, F = WT / 16;         // wave tile, fragments per side
-  static constexpr int L = T / 32;                      // LDS-DMA instructions per operand, wave and slab
-  static constexpr int PITCH = T + 4;                   // floats per row of the epilogue's tile
-  static constexpr int EPI = T * PITCH * 4;
-  static constexpr int LDS = NST * STAGE > EPI ? NST * STAGE : EPI;
+  static constexpr int OP = T * NS_BK * 2, STAGE = 2 * OP, RING = NST * STAGE;
+  static constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+  static constexpr int TM = T / WM, TN = T / WN, FM = TM / 16, FN = TN / 16;   // wave tile, fragments
+  static constexpr int L = T * 8 / (64 * WAVES);        // LDS-DMA instructions per operand, wave and slab
+  static constexpr int ER = T > 192 ? T / 2 : T;        // rows of one pass of the epilogue
+  static constexpr int PITCH = T + 4, EPI = ER * PITCH; // floats
+  static constexpr int LDS = RING > 4 * EPI ? RING : 4 * EPI;
   static __device__ __forceinline__ int block_xor(int row) {
-    return T == 128 ? (row & 3) | (((row >> 3) & 1) << 2) : ((row >> 1) & 1) | (((row >> 3) & 1) << 1);
+    return T % 128 == 0 ? (row & 3) | (((row >> 3) & 1) << 2) : ((row >> 1) & 1) | (((row >> 3) & 1) << 1);
   }
 
   static __device__ __forceinline__ void run(const NsGemm& g, int b, int tm, int tn, char* smem) {
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wr = wid >> 1, wc = wid & 1, fr = lane & 15, fq = lane >> 4;
-    const f16* A = g.A + b * g.bsa + (int64_t)tm * T * g.lda;
-    const f16* B = g.B + b * g.bsb + (MODE == NS_APPLY ? (int64_t)tn * T : (int64_t)tn * T * g.ldb);
-    const int arow = lane >> 3, achunk = ((lane & 7) ^ arow) * 8;
-    const f16* a_src = A + (int64_t)(wid * 8 + arow) * g.lda + achunk;
-    // APPLY: a wave instruction covers 1024 / (2 T) rows of the slab
-    constexpr int RI = 512 / T, CL = T / 8;
-    const f16* b_src;
-    if constexpr (MODE == NS_APPLY) {
-      // this wave's instructions are 4 RI rows apart: the XOR term is the same for all
-      const int row = wid * RI + lane / CL, pch = lane % CL;
-      b_src = B + (int64_t)row * g.ldb + (((pch >> 1) ^ block_xor(row)) * 2 + (pch & 1)) * 8;
-    } else {
-      b_src = B + (int64_t)(wid * 8 + arow) * g.ldb + achunk;
+    const int wr = wid / WN, wc = wid % WN, fr = lane & 15, fq = lane >> 4;
+    const int i0 = tm * T, j0 = tn * T;
+    const f16* A = g.A + b * g.bsa;
+    const f16* B = g.B + b * g.bsb;
+    unsigned aoff[L], boff[L];       // of this lane's 16 bytes of each instruction
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+      const int row = (i * WAVES + wid) * 8 + (lane >> 3), ch = ((lane & 7) ^ (row & 7)) * 8;
+      const int ai = i0 + row < g.M ? i0 + row : g.M - 1;
+      aoff[i] = (unsigned)((ai - i0) * (int)g.lda + ch);
+      if constexpr (MODE == NS_APPLY) {
+        const int q = (i * WAVES + wid) * 64 + lane, k = q / (T / 8), pch = q % (T / 8);
+        int j = j0 + (((pch >> 1) ^ block_xor(k)) * 2 + (pch & 1)) * 8;
+        j = j < g.N ? j : g.N - 8;
+        boff[i] = (unsigned)(k * (int)g.ldb + (j - j0));
+      } else {
+        const int bj = j0 + row < g.N ? j0 + row : g.N - 1;
+        boff[i] = (unsigned)((bj - j0) * (int)g.ldb + ch);
+      }
     }
+    A += (int64_t)i0 * g.lda;
+    B += MODE == NS_APPLY ? (int64_t)j0 : (int64_t)j0 * g.ldb;
     auto stage = [&](int st, int k0) {
       char* const sb = smem + st * STAGE;
+      const f16* a = A + k0;
+      const f16* bb = B + (MODE == NS_APPLY ? (int64_t)k0 * g.ldb : (int64_t)k0);
 #pragma unroll
       for (int i = 0; i < L; ++i) {
-        NS_GLDS16(a_src + (int64_t)(i * 32) * g.lda + k0, sb + (i * 4 + wid) * 1024);
-        if constexpr (MODE == NS_APPLY)
-          NS_GLDS16(b_src + (int64_t)(k0 + i * 4 * RI) * g.ldb, sb + OP + (i * 4 + wid) * 1024);
-        else
-          NS_GLDS16(b_src + (int64_t)(i * 32) * g.ldb + k0, sb + OP + (i * 4 + wid) * 1024);
+        NS_GLDS16(a + aoff[i], sb + (i * WAVES + wid) * 1024);
+        NS_GLDS16(bb + boff[i], sb + OP + (i * WAVES + wid) * 1024);
       }
     };
     int foff[2];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) foff[ks] = fr * 128 + (((ks * 4 + fq) ^ (lane & 7)) * 16);
-    const int a_base = wr * WT * 128, b_base = OP + wc * WT * 128;
-    unsigned tr[F];
+    const int a_base = wr * TM * 128, b_base = OP + wc * TN * 128;
+    unsigned tr[FN];
     if constexpr (MODE == NS_APPLY) {
       const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
       const int row = 8 * fq + (fr >> 2);       // + 4, + 32: the same XOR term
 #pragma unroll
-      for (int n = 0; n < F; ++n)
-        tr[n] = lds0 + OP + row * (2 * T) + (((wc * F + n) ^ block_xor(row)) * 32) + (lane & 3) * 8;
+      for (int n = 0; n < FN; ++n)
+        tr[n] = lds0 + OP + row * (2 * T) + (((wc * FN + n) ^ block_xor(row)) * 32) + (lane & 3) * 8;
     }
-    f32x4 acc[F][F];
+    f32x4 acc[FM][FN];
 #pragma unroll
-    for (int m = 0; m < F; ++m)
+    for (int m = 0; m < FM; ++m)
 #pragma unroll
-      for (int n = 0; n < F; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      for (int n = 0; n < FN; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
     const int KT = g.K / NS_BK;
+    auto read_a = [&](const char* sb, int ks, f16x8 (&f)[FM]) {
 #pragma unroll
-    for (int i = 0; i < NST - 1; ++i)
-      if (i < KT) stage(i, i * NS_BK);
-    int st = 0, st_in = NST - 1;      // ring slots read and filled next
-    for (int kt = 0; kt < KT; ++kt) {
-      const int behind = KT - 1 - kt;
-      slab_wait<2 * L>(behind < NST - 2 ? behind : NST - 2);
-      if (kt + NST - 1 < KT) stage(st_in, (kt + NST - 1) * NS_BK);
-      const char* sb = smem + st * STAGE;
-      f16x8 af[2][F], bf[2][F];
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int m = 0; m < F; ++m) af[ks][m] = *reinterpret_cast<const f16x8*>(sb + a_base + m * 2048 + foff[ks]);
-      if constexpr (MODE == NS_APPLY) {
-        // the reads and their wait in one block: the compiler does not count them
-        uint2 t[2][F][2];
-        const unsigned o = st * STAGE;
-        if constexpr (F == 4) {
-          const unsigned a0 = tr[0] + o, a1 = tr[1] + o, a2 = tr[2] + o, a3 = tr[3] + o;
-          asm volatile(
-            "ds_read_b64_tr_b16 %0, %16\n\tds_read_b64_tr_b16 %1, %16 offset:1024\n\t"
-            "ds_read_b64_tr_b16 %2, %17\n\tds_read_b64_tr_b16 %3, %17 offset:1024\n\t"
-            "ds_read_b64_tr_b16 %4, %18\n\tds_read_b64_tr_b16 %5, %18 offset:1024\n\t"
-            "ds_read_b64_tr_b16 %6, %19\n\tds_read_b64_tr_b16 %7, %19 offset:1024\n\t"
-            "ds_read_b64_tr_b16 %8, %16 offset:8192\n\tds_read_b64_tr_b16 %9, %16 offset:9216\n\t"
-            "ds_read_b64_tr_b16 %10, %17 offset:8192\n\tds_read_b64_tr_b16 %11, %17 offset:9216\n\t"
-            "ds_read_b64_tr_b16 %12, %18 offset:8192\n\tds_read_b64_tr_b16 %13, %18 offset:9216\n\t"
-            "ds_read_b64_tr_b16 %14, %19 offset:8192\n\tds_read_b64_tr_b16 %15, %19 offset:9216\n\t"
-            "s_waitcnt lgkmcnt(0)"
-            : "=&v"(t[0][0][0]), "=&v"(t[0][0][1]), "=&v"(t[0][1][0]), "=&v"(t[0][1][1]), "=&v"(t[0][2][0]),
-              "=&v"(t[0][2][1]), "=&v"(t[0][3][0]), "=&v"(t[0][3][1]), "=&v"(t[1][0][0]), "=&v"(t[1][0][1]),
-              "=&v"(t[1][1][0]), "=&v"(t[1][1][1]), "=&v"(t[1][2][0]), "=&v"(t[1][2][1]), "=&v"(t[1][3][0]),
-              "=&v"(t[1][3][1])
-            : "v"(a0), "v"(a1), "v"(a2), "v"(a3) : "memory");
-        } else {
-          const unsigned a0 = tr[0] + o, a1 = tr[1] + o;
-          asm volatile(
-            "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:512\n\t"
-            "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:512\n\t"
-            "ds_read_b64_tr_b16 %4, %8 offset:4096\n\tds_read_b64_tr_b16 %5, %8 offset:4608\n\t"
-            "ds_read_b64_tr_b16 %6, %9 offset:4096\n\tds_read_b64_tr_b16 %7, %9 offset:4608\n\t"
-            "s_waitcnt lgkmcnt(0)"
-            : "=&v"(t[0][0][0]), "=&v"(t[0][0][1]), "=&v"(t[0][1][0]), "=&v"(t[0][1][1]), "=&v"(t[1][0][0]),
-              "=&v"(t[1][0][1]), "=&v"(t[1][1][0]), "=&v"(t[1][1][1])
-            : "v"(a0), "v"(a1) : "memory");
-        }
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int n = 0; n < F; ++n)
-            bf[ks][n] = __builtin_bit_cast(f16x8, make_uint4(t[ks][n][0].x, t[ks][n][0].y, t[ks][n][1].x, t[ks][n][1].y));
-      } else {
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int n = 0; n < F; ++n) bf[ks][n] = *reinterpret_cast<const f16x8*>(sb + b_base + n * 2048 + foff[ks]);
-      }
-      // swapped operands: a lane holds four consecutive columns of one output row
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-        for (int m = 0; m < F; ++m)
-#pragma unroll
-          for (int n = 0; n < F; ++n)
-            acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf[ks][n], af[ks][m], acc[m][n], 0, 0, 0);
-      st = st + 1 == NST ? 0 : st + 1;
-      st_in = st_in + 1 == NST ? 0 : st_in + 1;
-    }
-    // ---- epilogue: the sums through LDS, so that global rows are read and written whole
-    __syncthreads();
-    float* const tile = reinterpret_cast<float*>(smem);
-#pragma unroll
-    for (int m = 0; m < F; ++m)
-#pragma unroll
-      for (int n = 0; n < F; ++n)
-        *reinterpret_cast<f32x4*>(tile + (wr * WT + m * 16 + fr) * PITCH + wc * WT + n * 16 + fq * 4) = acc[m][n];
-    __syncthreads();
-    const int i0 = tm * T, j0 = tn * T;
-    // eight outputs at (i, j..j+7)
-    auto put = [&](int i, int j, const float (&v)[8]) {
-      const int64_t at = b * g.bso + (int64_t)i * g.ldo + j;
-      f16x8 hv;
-      if constexpr (MODE == NS_GRAM) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float x = v[e] * (NS_SD / (NS_SX * NS_SX));
-          if (i == j + e) x += g.shift * NS_SD;
-          hv[e] = (f16)x;
-          if (i == j + e) g.diag[b * g.sp + i] = x - (float)hv[e];
-        }
-        *reinterpret_cast<f16x8*>(g.out + at) = hv;
-      } else {   // NS_SQUARE
-        const f16x8 dv = *reinterpret_cast<const f16x8*>(g.A + at);
-        const float di = g.diag[b * g.sp + i];
-        const f32x4 d0 = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j);
-        const f32x4 d1 = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j + 4);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float x = (v[e] + (di + (e < 4 ? d0[e & 3] : d1[e & 3])) * (float)dv[e]) * (g.c / NS_SD);
-          if (i == j + e) x += g.mu * NS_SD;      // (a - b^2/4c) - mu
-          hv[e] = (f16)x;
-        }
-        *reinterpret_cast<f16x8*>(g.out + at) = hv;
-      }
+      for (int m = 0; m < FM; ++m) f[m] = *reinterpret_cast<const f16x8*>(sb + a_base + m * 2048 + foff[ks]);
     };
-    constexpr int CH = T / 8, RP = 256 / CH;            // chunks of 8 per row, rows per pass
-    const int pr = tid / CH, pc = (tid % CH) * 8;
+    auto read_b = [&](const char* sb, int ks, f16x8 (&f)[FN]) {
 #pragma unroll
-    for (int r = 0; r < T; r += RP) {
-      const int i = r + pr;
-      const f32x4 lo4 = *reinterpret_cast<const f32x4*>(tile + i * PITCH + pc);
-      const f32x4 hi4 = *reinterpret_cast<const f32x4*>(tile + i * PITCH + pc + 4);
-      const float v[8] = {lo4[0], lo4[1], lo4[2], lo4[3], hi4[0], hi4[1], hi4[2], hi4[3]};
-      if constexpr (MODE != NS_APPLY) {
-        put(i0 + i, j0 + pc, v);
-      } else {
-        const int64_t at = b * g.bso + (int64_t)(i0 + i) * g.ldo + j0 + pc;
-        const f16x8 xh = *reinterpret_cast<const f16x8*>(g.B + at), xl = *reinterpret_cast<const f16x8*>(g.lo + at);
+      for (int n = 0; n < FN; ++n) f[n] = *reinterpret_cast<const f16x8*>(sb + b_base + n * 2048 + foff[ks]);
+    };
+    // swapped operands: a lane holds four consecutive columns of one output row
+    auto mma = [&](const f16x8 (&fa)[FM], const f16x8 (&fb)[FN]) {
+#pragma unroll
+      for (int m = 0; m < FM; ++m)
+#pragma unroll
+        for (int n = 0; n < FN; ++n)
+          acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[n], fa[m], acc[m][n], 0, 0, 0);
+    };
+    if constexpr (MODE != NS_APPLY) {
+#pragma unroll
+      for (int i = 0; i < NST; ++i)
+        if (i < KT) stage(i, i * NS_BK);
+      slab_wait<2 * L, NST - 1>(KT - 1);
+      f16x8 a0[FM], b0[FN], a1[FM], b1[FN];
+      read_a(smem, 0, a0);
+      read_b(smem, 0, b0);
+      int st = 0, kt = 0;
+      // a round: the second half's fragments are read under the first half's products,
+      // the next slab's first half and its DMA under the second half's (left to itself
+      // the compiler puts all reads and one wait in front: 10 - 20 % slower)
+      for (; kt + NST < KT; ++kt) {
+        const char* sb = smem + st * STAGE;
+        read_a(sb, 1, a1);
+        read_b(sb, 1, b1);
+        mma(a0, b0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+#pragma unroll
+        for (int i = 0; i < FM + FN; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NST - 2) * 2 * L) : "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        stage(st, (kt + NST) * NS_BK);
+        st = st + 1 == NST ? 0 : st + 1;
+        sb = smem + st * STAGE;
+        read_a(sb, 0, a0);
+        read_b(sb, 0, b0);
+        mma(a1, b1);
+#pragma unroll
+        for (int i = 0; i < FM + FN; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      for (; kt < KT; ++kt) {          // the last NST slabs: nothing left to fetch
+        read_a(smem + st * STAGE, 1, a1);
+        read_b(smem + st * STAGE, 1, b1);
+        mma(a0, b0);
+        st = st + 1 == NST ? 0 : st + 1;
+        if (kt + 1 < KT) {
+          slab_wait<2 * L, NST - 2>(KT - 2 - kt);
+          read_a(smem + st * STAGE, 0, a0);
+          read_b(smem + st * STAGE, 0, b0);
+        }
+        mma(a1, b1);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NST - 1; ++i)
+        if (i < KT) stage(i, i * NS_BK);
+      int st = 0, st_in = NST - 1;      // ring slots read and filled next
+      for (int kt = 0; kt < KT; ++kt) {
+        slab_wait<2 * L, NST - 2>(KT - 1 - kt);
+        if (kt + NST - 1 < KT) stage(st_in, (kt + NST - 1) * NS_BK);
+        const char* sb = smem + st * STAGE;
+        f16x8 af[2][FM], bf[2][FN];
+        read_a(sb, 0, af[0]);
+        read_a(sb, 1, af[1]);
+        // the reads and their wait in one block: the compiler does not count them
+        uint2 t[2][FN][2];
+        const unsigned o = st * STAGE;
+#define TR4(d0, d1, d2, d3, a)                                                              \
+  "ds_read_b64_tr_b16 %" #d0 ", %" #a "\n\tds_read_b64_tr_b16 %" #d1 ", %" #a " offset:%c[o4]\n\t" \
+  "ds_read_b64_tr_b16 %" #d2 ", %" #a " offset:%c[o32]\n\tds_read_b64_tr_b16 %" #d3 ", %" #a " offset:%c[o36]\n\t"
+#define TRO(n) "=&v"(t[0][n][0]), "=&v"(t[0][n][1]), "=&v"(t[1][n][0]), "=&v"(t[1][n][1])
+#define TRC [o4] "n"(4 * 2 * T), [o32] "n"(32 * 2 * T), [o36] "n"(36 * 2 * T)
+        if constexpr (FN == 4)
+          asm volatile(TR4(0, 1, 2, 3, 16) TR4(4, 5, 6, 7, 17) TR4(8, 9, 10, 11, 18) TR4(12, 13, 14, 15, 19)
+                       "s_waitcnt lgkmcnt(0)"
+                       : TRO(0), TRO(1), TRO(2), TRO(3)
+                       : "v"(tr[0] + o), "v"(tr[1] + o), "v"(tr[2] + o), "v"(tr[3] + o), TRC : "memory");
+        else if constexpr (FN == 3)
+          asm volatile(TR4(0, 1, 2, 3, 12) TR4(4, 5, 6, 7, 13) TR4(8, 9, 10, 11, 14) "s_waitcnt lgkmcnt(0)"
+                       : TRO(0), TRO(1), TRO(2)
+                       : "v"(tr[0] + o), "v"(tr[1] + o), "v"(tr[2] + o), TRC : "memory");
+        else
+          asm volatile(TR4(0, 1, 2, 3, 8) TR4(4, 5, 6, 7, 9) "s_waitcnt lgkmcnt(0)"
+                       : TRO(0), TRO(1)
+                       : "v"(tr[0] + o), "v"(tr[1] + o), TRC : "memory");
+#undef TR4
+#undef TRO
+#undef TRC
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int n = 0; n < FN; ++n)
+            bf[ks][n] = __builtin_bit_cast(f16x8, make_uint4(t[ks][n][0].x, t[ks][n][0].y, t[ks][n][1].x, t[ks][n][1].y));
+        mma(af[0], bf[0]);
+        mma(af[1], bf[1]);
+        st = st + 1 == NST ? 0 : st + 1;
+        st_in = st_in + 1 == NST ? 0 : st_in + 1;
+      }
+    }
+
+    // ---- epilogue: the sums through LDS, so that global rows are read and written whole.
+    // What an output needs from memory is fetched before the sums are turned round.
+    float* const tile = reinterpret_cast<float*>(smem);
+    // the other side of a symmetric product, or a tall matrix's own orientation
+    const bool turn = MODE == NS_APPLY ? g.last && g.tall : tm != tn;
+    constexpr int CH = T / 8, NC = ER * CH / THREADS > 0 ? ER * CH / THREADS : 1;      // chunks of 8: per row, per thread
+    static_assert(NC * THREADS == ER * CH || ER * CH < THREADS, "whole chunks per thread");
+#pragma unroll
+    for (int part = 0; part < T / ER; ++part) {
+      const int ip = i0 + part * ER;
+      f16x8 ga[NC], gb[NC];
+      bool ok[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int q = tid + c * THREADS, i = ip + q / CH, j = j0 + q % CH * 8;
+        ok[c] = q < ER * CH && i < g.M && j < g.N;
+        if (MODE != NS_GRAM && ok[c]) {
+          const int64_t at = b * g.bso + (int64_t)i * g.ldo + j;
+          ga[c] = *reinterpret_cast<const f16x8*>((MODE == NS_SQUARE ? g.A : g.B) + at);
+          if (MODE == NS_APPLY) gb[c] = *reinterpret_cast<const f16x8*>(g.lo + at);
+        }
+      }
+      __syncthreads();
+      if (T == ER || wr * TM / ER == part) {
+        float* const own = tile + (wr * TM - part * ER) * PITCH;
+#pragma unroll
+        for (int m = 0; m < FM; ++m)
+#pragma unroll
+          for (int n = 0; n < FN; ++n)
+            *reinterpret_cast<f32x4*>(own + (m * 16 + fr) * PITCH + wc * TN + n * 16 + fq * 4) = acc[m][n];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if (!ok[c]) continue;
+        const int q = tid + c * THREADS, r = q / CH, pc = q % CH * 8, i = ip + r, j = j0 + pc;
+        const int64_t at = b * g.bso + (int64_t)i * g.ldo + j;
+        f32x4* const t4 = reinterpret_cast<f32x4*>(tile + r * PITCH + pc);
+        const f32x4 v0 = t4[0], v1 = t4[1];
         float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = g.mu * ((float)xh[e] + (float)xl[e]) + v[e] * (1.f / NS_SD);
-        if (!g.last) {
-          f16x8 hv, lv;
+        for (int e = 0; e < 8; ++e) x[e] = e < 4 ? v0[e & 3] : v1[e & 3];
+        const int on_diag = i - j;                 // 0..7: element of the chunk on the diagonal
+        if constexpr (MODE == NS_GRAM) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) { f16 hh, ll; split_f16(x[e], hh, ll); hv[e] = hh; lv[e] = ll; }
-          *reinterpret_cast<f16x8*>(g.out + at) = hv;
-          *reinterpret_cast<f16x8*>(g.lo + at) = lv;
-        } else {
+          for (int e = 0; e < 8; ++e) x[e] *= NS_SD / (NS_SX * NS_SX);
+          if (on_diag >= 0 && on_diag < 8) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] *= 1.f / NS_SX;
-          if (!g.tall) {
-            ns_store8(g.dst, b, i0 + i, j0 + pc, x);
-          } else {
-            *reinterpret_cast<f32x4*>(tile + i * PITCH + pc) = (f32x4){x[0], x[1], x[2], x[3]};
-            *reinterpret_cast<f32x4*>(tile + i * PITCH + pc + 4) = (f32x4){x[4], x[5], x[6], x[7]};
+            for (int e = 0; e < 8; ++e)
+              if (e == on_diag) {
+                x[e] += g.shift * NS_SD;
+                g.diag[b * g.sp + i] = x[e] - (float)(f16)x[e];
+              }
           }
+        } else if constexpr (MODE == NS_SQUARE) {
+          const float di = g.diag[b * g.sp + i];
+          const f32x4 d0 = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j);
+          const f32x4 d1 = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j + 4);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            x[e] = (x[e] + (di + (e < 4 ? d0[e & 3] : d1[e & 3])) * (float)ga[c][e]) * (g.c / NS_SD);
+          if (on_diag >= 0 && on_diag < 8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) if (e == on_diag) x[e] += g.mu * NS_SD;      // (a - b^2/4c) - mu
+          }
+        } else {
+          const float sc = g.last ? 1.f / NS_SX : 1.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            x[e] = (g.mu * ((float)ga[c][e] + (float)gb[c][e]) + x[e] * (1.f / NS_SD)) * sc;
+        }
+        if (turn) { t4[0] = (f32x4){x[0], x[1], x[2], x[3]}; t4[1] = (f32x4){x[4], x[5], x[6], x[7]}; }
+        if (MODE == NS_APPLY && g.last) {
+          if (!turn) ns_store8(g.dst, b, i, j, x);
+          continue;
+        }
+        f16x8 hv;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) hv[e] = (f16)x[e];
+        *reinterpret_cast<f16x8*>(g.out + at) = hv;
+        if constexpr (MODE == NS_APPLY) {
+          f16x8 lv;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) lv[e] = (f16)(x[e] - (float)hv[e]);
+          *reinterpret_cast<f16x8*>(g.lo + at) = lv;
         }
       }
-    }
-    // the other side of a symmetric product, or a tall matrix's own orientation:
-    // 16 columns x 4 chunks of 8 rows per wave and pass
-    const bool turn = MODE == NS_APPLY ? g.last && g.tall : tm != tn;
-    if (turn) {
-      if constexpr (MODE == NS_APPLY) __syncthreads();
+      if (turn) {      // 16 columns x 4 chunks of 8 rows per wave and pass
+        __syncthreads();
+        constexpr int UNITS = (T / 16) * (ER / 32);
 #pragma unroll 4
-      for (int q = wid; q < (T / 16) * (T / 32); q += 4) {
-        const int j = (q % (T / 16)) * 16 + fr, i = (q / (T / 16)) * 32 + fq * 8;
-        float v[8];
+        for (int q = wid; q < UNITS; q += WAVES) {
+          const int jj = (q % (T / 16)) * 16 + fr, ii = (q / (T / 16)) * 32 + fq * 8;
+          const int i = ip + ii, j = j0 + jj;
+          if (i >= g.M || j >= g.N) continue;
+          float x[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = tile[(i + e) * PITCH + j];
-        if constexpr (MODE == NS_APPLY) ns_store8(g.dst, b, j0 + j, i0 + i, v);
-        else put(j0 + j, i0 + i, v);
+          for (int e = 0; e < 8; ++e) x[e] = tile[(ii + e) * PITCH + jj];
+          if constexpr (MODE == NS_APPLY) {
+            ns_store8(g.dst, b, j, i, x);
+          } else {
+            f16x8 hv;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) hv[e] = (f16)x[e];
+            *reinterpret_cast<f16x8*>(g.out + b * g.bso + (int64_t)j * g.ldo + i) = hv;
+          }
+        }
       }
     }
   }
@@ -474,10 +548,10 @@ __device__ __forceinline__ void triangle(int t, int& tm, int& tn) {
   tn = t - tm * (tm + 1) / 2;
 }
 
-template <int MODE, int T, int NST>
-__global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsGemm g) {
+template <int MODE, int T, int WM, int WN, int NST>
+__global__ __launch_bounds__(64 * WM * WN, T <= 128 ? 2 : WM * WN / 4) void ns_gemm_kernel(NsGemm g) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int tiles_m = g.M / T, tiles_n = g.N / T;
+  const int tiles_m = (g.M + T - 1) / T, tiles_n = (g.N + T - 1) / T;
   const int per_mat = MODE == NS_APPLY ? tiles_m * tiles_n : tiles_m * (tiles_m + 1) / 2, total = per_mat * g.n;
   // each XCD (workgroup id & 7) gets a contiguous range of tiles
   const int per_xcd = (total + 7) >> 3;
@@ -487,31 +561,59 @@ __global__ __launch_bounds__(256, 2) void ns_gemm_kernel(NsGemm g) {
   int tm, tn;
   if (MODE == NS_APPLY) { tn = t / tiles_m; tm = t - tn * tiles_m; }     // X's columns are read once per XCD
   else triangle(t, tm, tn);
-  NsTile<MODE, T, NST>::run(g, b, tm, tn, smem);
+  NsTile<MODE, T, WM, WN, NST>::run(g, b, tm, tn, smem);
 }
 
-template <int MODE, int T, int NST>
+static int64_t ns_tiles(int mode, const NsGemm& g, int T) {
+  const int64_t tm = (g.M + T - 1) / T, tn = (g.N + T - 1) / T;
+  return (mode == NS_APPLY ? tm * tn : tm * (tm + 1) / 2) * g.n;
+}
+template <int MODE, int T, int WM, int WN, int NST>
 static int ns_launch(const NsGemm& g, hipStream_t st) {
-  constexpr int LDS = NsTile<MODE, T, NST>::LDS;
+  constexpr int LDS = NsTile<MODE, T, WM, WN, NST>::LDS;
+  static_assert(LDS <= 160 * 1024, "LDS of a CU");
   static bool done[MAX_DEVICES] = {};
-  if (int rc = ensure_dynamic_lds(&ns_gemm_kernel<MODE, T, NST>, LDS, done, "orthogonalize")) return rc;
-  const int64_t tm = g.M / T, tn = g.N / T, total = (MODE == NS_APPLY ? tm * tn : tm * (tm + 1) / 2) * g.n;
+  if (int rc = ensure_dynamic_lds(&ns_gemm_kernel<MODE, T, WM, WN, NST>, LDS, done, "orthogonalize")) return rc;
+  const int64_t total = ns_tiles(MODE, g, T);
   if (total >= (1ll << 28)) { set_error("orthogonalize: too many tiles"); return -1; }
-  ns_gemm_kernel<MODE, T, NST><<<(unsigned)((total + 7) / 8 * 8), 256, LDS, st>>>(g);
+  ns_gemm_kernel<MODE, T, WM, WN, NST><<<(unsigned)((total + 7) / 8 * 8), 64 * WM * WN, LDS, st>>>(g);
   MDLM_LAUNCH_CHECK();
   return 0;
 }
+// Which tile.  Up to 256 tiles of 128 x 128 (one per CU) the smaller 64 x 64 ones fill the
+// chip better; their ring is deep (4 slabs) while a CU holds at most two of them and
+// shallow (2 slabs, five workgroups per CU) beyond.  Measured, us per product:
+//   A of 768 x 768:            64: 6.2 / 8.9 (deep / shallow)   128: 13
+//   A of 1024 x 4096:          64: 16 / 30                      128: 41
+//   A of 2048 x 2048:          64: 22 / 19                      128: 25
+// With more, the rounds of tiles that a CU goes through, times what a slab of one
+// costs with the chip full (us, measured on 4096 x 4096: 128: 0.59 in pairs, 192:
+// 1.16, 256: 1.5; P X: 128: 0.54, 256: 2.0):
+//   A of 4096 x 8192:          128: 196   192: 139   256: 179
+//   A of 24 x 1024 x 4096:     128: 139   192: 140   256: 121
+//   P X of 24 x 1024 x 4096:   128: 353   256: 303
+//   P X of 12 x 768 x 2304:    128: 52    256: 68
 template <int MODE>
-static int ns_gemm(const NsGemm& g, hipStream_t st) {
-  const int64_t tm = g.M / 128, tn = g.N / 128;
-  const int64_t tiles = (MODE == NS_APPLY ? tm * tn : tm * (tm + 1) / 2) * g.n;
-  if (g.M % 128 || g.N % 128 || tiles < NS_FEW_TILES) return ns_launch<MODE, 64, 4>(g, st);
-  return ns_launch<MODE, 128, 2>(g, st);
+static int ns_gemm(const NsGemm& g, int cus, hipStream_t st) {
+  const int64_t t128 = ns_tiles(MODE, g, 128);
+  if (t128 <= cus)
+    return ns_tiles(MODE, g, 64) <= 2 * cus ? ns_launch<MODE, 64, 2, 2, 4>(g, st) : ns_launch<MODE, 64, 2, 2, 2>(g, st);
+  auto rounds = [&](int T, int slots) { return (double)((ns_tiles(MODE, g, T) + slots - 1) / slots); };
+  const double c128 = rounds(128, 2 * cus) * 2 * (MODE == NS_APPLY ? 0.54 : 0.59);
+  const double c256 = rounds(256, cus) * (MODE == NS_APPLY ? 2.0 : 1.5);
+  if constexpr (MODE != NS_APPLY) {
+    const double c192 = rounds(192, cus) * 1.16;
+    if (c192 < c128 && c192 <= c256) return ns_launch<MODE, 192, 2, 4, 3>(g, st);
+  }
+  return c256 < c128 ? ns_launch<MODE, 256, 2, 4, 2>(g, st) : ns_launch<MODE, 128, 2, 2, 2>(g, st);
 }
 
 static int ns_run(const NsSrc& src, NsOut dst, int n, int rows, int cols, int steps, double a, double b, double c,
                   double eps, void* ws, hipStream_t st) {
-  const NsShape q = ns_shape(n, rows, cols);
+  const int dev = current_device();
+  if (dev < 0) return -1;
+  const int cus = device_cus(dev);
+  const NsShape q = ns_shape(rows, cols);
   NsWs w;
   ns_layout(q, n, (char*)ws, &w);
   dst.rows = rows; dst.cols = cols;
@@ -531,14 +633,14 @@ static int ns_run(const NsSrc& src, NsOut dst, int n, int rows, int cols, int st
     g.A = x; g.lda = q.lp; g.bsa = bx; g.B = x; g.ldb = q.lp; g.bsb = bx; g.K = q.lp;
     g.M = g.N = q.sp;
     g.out = w.d; g.ldo = q.sp; g.bso = bd; g.shift = (float)(b / (2 * c));
-    if (int rc = ns_gemm<NS_GRAM>(g, st)) return rc;
+    if (int rc = ns_gemm<NS_GRAM>(g, cus, st)) return rc;
     g.A = w.d; g.lda = q.sp; g.bsa = bd; g.B = w.d; g.ldb = q.sp; g.bsb = bd; g.K = q.sp;
     g.out = w.p; g.c = (float)c; g.mu = (float)(a - b * b / (4 * c) - mu);
-    if (int rc = ns_gemm<NS_SQUARE>(g, st)) return rc;
+    if (int rc = ns_gemm<NS_SQUARE>(g, cus, st)) return rc;
     g.A = w.p; g.B = x; g.ldb = q.lp; g.bsb = bx; g.N = q.lp;
     g.out = xn; g.ldo = q.lp; g.bso = bx; g.lo = w.lo; g.mu = (float)mu;
     g.last = it + 1 == steps; g.tall = q.tall; g.dst = dst;
-    if (int rc = ns_gemm<NS_APPLY>(g, st)) return rc;
+    if (int rc = ns_gemm<NS_APPLY>(g, cus, st)) return rc;
   }
   return 0;
 }
@@ -564,7 +666,7 @@ using namespace mdlm;
 
 extern "C" int64_t mdlm_orthogonalize_workspace_bytes(int n, int rows, int cols) {
   if (n <= 0 || rows <= 0 || cols <= 0 || n >= 65536 || rows > (1 << 17) || cols > (1 << 17)) return -1;
-  return ns_layout(ns_shape(n, rows, cols), n, nullptr, nullptr);
+  return ns_layout(ns_shape(rows, cols), n, nullptr, nullptr);
 }
 
 extern "C" int mdlm_orthogonalize(const void* g, int64_t ldg, int64_t g_stride, int dtype, void* out_bf16, int64_t ldo,

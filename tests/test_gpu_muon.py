@@ -68,6 +68,17 @@ def test_orthogonalize(ops, n, r, c, dtype):
       assert rel(got[i], want[i]) < tol_factor(5) + 2.0 ** -8, (i, decay)
 
 
+@pytest.mark.parametrize('n,r,c', [(300, 100, 140), (40, 560, 600), (25, 1000, 990), (30, 1100, 300)])
+def test_orthogonalize_many_matrices(ops, n, r, c):
+  """Stacks large enough for the larger tiles.  Every tile adds the same products in the
+  same order, so a matrix's result does not depend on the company it is in."""
+  g = gradient(n, r, c, seed=n).to(torch.bfloat16).cuda()
+  got = ops.orthogonalize(g)
+  for i in (0, n // 2, n - 1):
+    assert torch.equal(got[i], ops.orthogonalize(g[i])), i
+  assert rel(got[n - 1], oracle(g[n - 1])) < tol_factor(5) + 2.0 ** -8
+
+
 @pytest.mark.parametrize('coeffs', [COEFFS, (1.875, -1.25, 0.375), (2.0, -1.5, 0.5)])
 @pytest.mark.parametrize('steps', [1, 2, 3, 7])
 def test_orthogonalize_steps_and_coefficients(ops, steps, coeffs):
