@@ -30,7 +30,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NS_BK = 64;
-constexpr int NS_NORM_BLOCKS = 256;   // partial sums of |G|^2 per matrix
+constexpr int NS_MAX_PARTS = 1024;    // partial sums of |G|^2 per matrix, at most
 // Powers of two that keep the fp16 words away from the subnormal range: entries
 // of X are at most about 1.2 and about 1/sqrt(s l) on average, D and P are at
 // most a few units.
@@ -51,7 +51,7 @@ static inline NsShape ns_shape(int rows, int cols) {
 
 // workspace of n matrices
 struct NsWs {
-  double* norm;      // n x NS_NORM_BLOCKS partial sums of squares
+  double* norm;      // n x NS_MAX_PARTS partial sums of squares
   float* diag;       // n x sp
   f16 *h[2], *lo;    // n x sp x lp
   f16 *d, *p;        // n x sp x sp
@@ -61,7 +61,7 @@ static inline int64_t ns_layout(const NsShape& q, int n, char* base, NsWs* w) {
   auto take = [&](int64_t bytes) { const int64_t at = off; off += (bytes + 255) / 256 * 256; return base + at; };
   const int64_t x = (int64_t)n * q.sp * q.lp, d = (int64_t)n * q.sp * q.sp;
   NsWs t;
-  t.norm = (double*)take((int64_t)n * NS_NORM_BLOCKS * 8);
+  t.norm = (double*)take((int64_t)n * NS_MAX_PARTS * 8);
   t.diag = (float*)take((int64_t)n * q.sp * 4);
   t.h[0] = (f16*)take(x * 2);
   t.h[1] = (f16*)take(x * 2);
@@ -76,6 +76,7 @@ static inline int64_t ns_layout(const NsShape& q, int n, char* base, NsWs* w) {
 // of the clipped gradient.
 struct NsSrc {
   const void* g; int64_t ld, bs; int bf16;
+  int rows, cols, vec;      // vec: rows start 16-byte aligned
   float* m;                 // momentum, the layout of g (null: g alone)
   float momentum;
   const float* sumsq; float max_norm, grad_scale;
@@ -88,73 +89,130 @@ __device__ __forceinline__ float clip_coef(const NsSrc& a) {
   }
   return coef;
 }
-__device__ __forceinline__ float src_load(const NsSrc& a, int64_t i, float coef) {
-  float g = a.bf16 ? bf16_to_f32(((const bf16_t*)a.g)[i]) : ((const float*)a.g)[i];
-  if (a.m) {
-    g *= coef;
-    g += a.momentum * (a.m[i] - g);
+// eight columns of row r of matrix b, from column c (a multiple of 8) on; 0 past the last.
+// STEP: the momentum is moved first (the one pass that does so comes before the others).
+template <bool STEP>
+__device__ __forceinline__ void src_load8(const NsSrc& a, int b, int r, int c, float coef, float (&v)[8]) {
+  const int64_t at = b * a.bs + r * a.ld + c;
+  float g[8], m[8];
+  if (a.vec && c + 8 <= a.cols) {
+    if (a.bf16) {
+      const uint4 q = *reinterpret_cast<const uint4*>((const bf16_t*)a.g + at);
+      const unsigned u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[e] = __uint_as_float(e & 1 ? u[e >> 1] & 0xffff0000u : u[e >> 1] << 16);
+    } else {
+      const float4 x = *reinterpret_cast<const float4*>((const float*)a.g + at);
+      const float4 y = *reinterpret_cast<const float4*>((const float*)a.g + at + 4);
+      g[0] = x.x; g[1] = x.y; g[2] = x.z; g[3] = x.w; g[4] = y.x; g[5] = y.y; g[6] = y.z; g[7] = y.w;
+    }
+    if (a.m) {
+      const float4 x = *reinterpret_cast<const float4*>(a.m + at), y = *reinterpret_cast<const float4*>(a.m + at + 4);
+      m[0] = x.x; m[1] = x.y; m[2] = x.z; m[3] = x.w; m[4] = y.x; m[5] = y.y; m[6] = y.z; m[7] = y.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool in = c + e < a.cols;
+      g[e] = !in ? 0.f : a.bf16 ? bf16_to_f32(((const bf16_t*)a.g)[at + e]) : ((const float*)a.g)[at + e];
+      m[e] = in && a.m ? a.m[at + e] : 0.f;
+    }
   }
-  return g;
+  if (!a.m) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = g[e];
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    g[e] *= coef;
+    if (STEP) m[e] = m[e] + (g[e] - m[e]) * (1.f - a.momentum);
+    v[e] = g[e] + a.momentum * (m[e] - g[e]);
+  }
+  if (STEP) {
+    if (a.vec && c + 8 <= a.cols) {
+      *reinterpret_cast<float4*>(a.m + at) = make_float4(m[0], m[1], m[2], m[3]);
+      *reinterpret_cast<float4*>(a.m + at + 4) = make_float4(m[4], m[5], m[6], m[7]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e < a.cols) a.m[at + e] = m[e];
+    }
+  }
 }
 
 // momentum (in place) and the partial sums of squares of what will be orthogonalised,
 // in 64 bits: squares of small gradients leave the fp32 range
-__global__ __launch_bounds__(256) void ns_norm_kernel(NsSrc a, double* __restrict__ part, int rows, int cols) {
+__global__ __launch_bounds__(256) void ns_norm_kernel(NsSrc a, double* __restrict__ part) {
   __shared__ double red[4];
   const int b = blockIdx.y;
   const float coef = a.m ? clip_coef(a) : 1.f;
+  const unsigned per_row = (a.cols + 7) / 8, chunks = per_row * a.rows, step = gridDim.x * 256;
   double acc = 0.0;
-  for (int r = blockIdx.x; r < rows; r += gridDim.x) {
-    const int64_t at = b * a.bs + r * a.ld;
-    for (int c = threadIdx.x; c < cols; c += 256) {
-      if (a.m) {
-        const float g = ((const float*)a.g)[at + c] * coef, m = a.m[at + c];
-        a.m[at + c] = m + (g - m) * (1.f - a.momentum);
-      }
-      const double u = src_load(a, at + c, coef);
-      acc += u * u;
-    }
+  for (unsigned q = blockIdx.x * 256 + threadIdx.x; q < chunks; q += step) {
+    const unsigned r = q / per_row;
+    float v[8];
+    src_load8<true>(a, b, r, (q - r * per_row) * 8, coef, v);
+    double s = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += (double)v[e] * (double)v[e];
+    acc += s;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
   __syncthreads();
-  if (threadIdx.x == 0) part[b * NS_NORM_BLOCKS + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+  if (threadIdx.x == 0) part[(int64_t)b * NS_MAX_PARTS + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-__device__ __forceinline__ void split_f16(float x, f16& h, f16& l) {
-  h = (f16)x;
-  l = (f16)(x - (float)h);
-}
-
-// X_0 = G / (|G| + eps), scaled, as hi + lo; 32 x 32 tiles through LDS so that a tall
-// G is read by rows and written by rows
-__global__ __launch_bounds__(256) void ns_ingest_kernel(NsSrc a, const double* __restrict__ part, double eps,
-                                                        f16* __restrict__ h, f16* __restrict__ lo, int rows, int cols,
-                                                        int sp, int lp, int tall) {
-  __shared__ float tile[32][33];
-  __shared__ float inv_s;
+// X_0 = G / (|G| + eps), scaled, as hi + lo, 64 x 64 at a time; a tall G goes through LDS,
+// so that it is read by rows and written by rows
+__global__ __launch_bounds__(256) void ns_ingest_kernel(NsSrc a, const double* __restrict__ part, int parts, double eps,
+                                                        f16* __restrict__ h, f16* __restrict__ lo, int sp, int lp,
+                                                        int tall) {
+  __shared__ float tile[64][65];
+  __shared__ double red[4];
   const int b = blockIdx.z, tid = threadIdx.x;
-  if (tid < 64) {
-    double t = 0.0;
-    for (int i = tid; i < NS_NORM_BLOCKS; i += 64) t += part[b * NS_NORM_BLOCKS + i];
+  const float coef = a.m ? clip_coef(a) : 1.f;
+  const int i0 = blockIdx.y * 64, j0 = blockIdx.x * 64;   // of X
+  float v[2][8];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o);
-    if (tid == 0) inv_s = (float)((double)NS_SX / (sqrt(t) + eps));
+  for (int k = 0; k < 2; ++k) {
+    const int q = tid + k * 256, y = q >> 3, x = (q & 7) * 8;
+    const int r = (tall ? j0 : i0) + y, c = (tall ? i0 : j0) + x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[k][e] = 0.f;
+    if (r < a.rows && c < a.cols) src_load8<false>(a, b, r, c, coef, v[k]);
   }
+  double t = 0.0;
+  for (int i = tid; i < parts; i += 256) t += part[(int64_t)b * NS_MAX_PARTS + i];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o);
+  if ((tid & 63) == 0) red[tid >> 6] = t;
   __syncthreads();
-  const float inv = inv_s, coef = a.m ? clip_coef(a) : 1.f;
-  const int i0 = blockIdx.y * 32, j0 = blockIdx.x * 32;   // of X
-  const int tx = tid & 31, ty = tid >> 5;
-  for (int k = ty; k < 32; k += 8) {
-    const int r = tall ? j0 + k : i0 + k, c = tall ? i0 + tx : j0 + tx;
-    const float v = r < rows && c < cols ? src_load(a, b * a.bs + r * a.ld + c, coef) * inv : 0.f;
-    if (tall) tile[tx][k] = v; else tile[k][tx] = v;
+  const float inv = (float)((double)NS_SX / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + eps));
+  if (tall) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int q = tid + k * 256, y = q >> 3, x = (q & 7) * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) tile[x + e][y] = v[k][e];
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  for (int k = ty; k < 32; k += 8) {
-    const int64_t at = ((int64_t)b * sp + i0 + k) * lp + j0 + tx;
-    split_f16(tile[k][tx], h[at], lo[at]);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int q = tid + k * 256, y = q >> 3, x = (q & 7) * 8;
+    f16x8 hv, lv;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float f = (tall ? tile[y][x + e] : v[k][e]) * inv;
+      hv[e] = (f16)f;
+      lv[e] = (f16)(f - (float)hv[e]);
+    }
+    const int64_t at = ((int64_t)b * sp + i0 + y) * lp + j0 + x;
+    *reinterpret_cast<f16x8*>(h + at) = hv;
+    *reinterpret_cast<f16x8*>(lo + at) = lv;
   }
 }
 
@@ -608,7 +666,7 @@ static int ns_gemm(const NsGemm& g, int cus, hipStream_t st) {
   return c256 < c128 ? ns_launch<MODE, 256, 2, 4, 2>(g, st) : ns_launch<MODE, 128, 2, 2, 2>(g, st);
 }
 
-static int ns_run(const NsSrc& src, NsOut dst, int n, int rows, int cols, int steps, double a, double b, double c,
+static int ns_run(NsSrc src, NsOut dst, int n, int rows, int cols, int steps, double a, double b, double c,
                   double eps, void* ws, hipStream_t st) {
   const int dev = current_device();
   if (dev < 0) return -1;
@@ -619,10 +677,15 @@ static int ns_run(const NsSrc& src, NsOut dst, int n, int rows, int cols, int st
   dst.rows = rows; dst.cols = cols;
   dst.vec = (dst.ld | dst.bs) % 8 == 0 &&
             (((uintptr_t)dst.out | (uintptr_t)dst.p | (uintptr_t)dst.ema | (uintptr_t)dst.w16) & 15) == 0;
-  ns_norm_kernel<<<dim3(NS_NORM_BLOCKS, n), 256, 0, st>>>(src, w.norm, rows, cols);
+  src.rows = rows; src.cols = cols;
+  src.vec = (src.ld | src.bs) % 8 == 0 && (((uintptr_t)src.g | (uintptr_t)src.m) & 15) == 0;
+  // some 2048 workgroups over all matrices, eight columns per thread and turn
+  const int64_t want = ((int64_t)rows * ((cols + 7) / 8) + 255) / 256, most = 2048 / n > 1 ? 2048 / n : 1;
+  int parts = (int)(want < most ? want : most);
+  if (parts > NS_MAX_PARTS) parts = NS_MAX_PARTS;
+  ns_norm_kernel<<<dim3(parts, n), 256, 0, st>>>(src, w.norm);
   MDLM_LAUNCH_CHECK();
-  const dim3 grid32(q.lp / 32, q.sp / 32, n);
-  ns_ingest_kernel<<<grid32, 256, 0, st>>>(src, w.norm, eps, w.h[0], w.lo, rows, cols, q.sp, q.lp, q.tall);
+  ns_ingest_kernel<<<dim3(q.lp / 64, q.sp / 64, n), 256, 0, st>>>(src, w.norm, parts, eps, w.h[0], w.lo, q.sp, q.lp, q.tall);
   MDLM_LAUNCH_CHECK();
   const int64_t bx = (int64_t)q.sp * q.lp, bd = (int64_t)q.sp * q.sp;
   for (int it = 0; it < steps; ++it) {
