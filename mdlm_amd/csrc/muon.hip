@@ -10,8 +10,10 @@
 // D = A + (b/2c) I is small near convergence and nothing cancels:
 //   P = c D D^T + (a - b^2/4c) I,   X <- mu X + (P - mu I) X.
 // mu = a in the early steps (small singular values: P is close to a I) and 1 in
-// the last two (P is close to I), and the mu X term takes X from TWO fp16 words
-// (hi + lo, 22 bits), so that only the small P - mu I sees X rounded to fp16.
+// the last two (P is close to I), and the mu X term takes X from two words, fp16 and
+// e4m3 (15 bits together: 16 more bits of the second word change nothing, and it is a
+// third of what the products move), so that only the small P - mu I sees X rounded
+// to fp16.  Without the second word matrices of fast decaying spectra lose: 3e-3.
 // The diagonal of D, its largest part, is also corrected for its rounding:
 // d = D_ii - fp16(D_ii) enters D D^T to first order.  Against 64 bits the result is
 // 4e-4 .. 1e-3 off (2-norm, relative), less than rounding it to bf16 costs
@@ -36,6 +38,7 @@ constexpr int NS_MAX_PARTS = 1024;    // partial sums of |G|^2 per matrix, at mo
 // most a few units.
 constexpr float NS_SX = 2048.f;
 constexpr float NS_SD = 256.f;
+constexpr float NS_SL = 16.f;         // of the second word: at most half a step of the first, 8 up to X = 2^14
 
 struct NsShape { int s, l, sp, lp; bool tall; };
 static inline NsShape ns_shape(int rows, int cols) {
@@ -53,7 +56,8 @@ static inline NsShape ns_shape(int rows, int cols) {
 struct NsWs {
   double* norm;      // n x NS_MAX_PARTS partial sums of squares
   float* diag;       // n x sp
-  f16 *h[2], *lo;    // n x sp x lp
+  f16* h[2];         // n x sp x lp, X's first words
+  uint8_t* lo;       // n x sp x lp, its second words
   f16 *d, *p;        // n x sp x sp
 };
 static inline int64_t ns_layout(const NsShape& q, int n, char* base, NsWs* w) {
@@ -65,7 +69,7 @@ static inline int64_t ns_layout(const NsShape& q, int n, char* base, NsWs* w) {
   t.diag = (float*)take((int64_t)n * q.sp * 4);
   t.h[0] = (f16*)take(x * 2);
   t.h[1] = (f16*)take(x * 2);
-  t.lo = (f16*)take(x * 2);
+  t.lo = (uint8_t*)take(x);
   t.d = (f16*)take(d * 2);
   t.p = (f16*)take(d * 2);
   if (w) *w = t;
@@ -165,10 +169,24 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsSrc a, double* __restric
   if (threadIdx.x == 0) part[(int64_t)b * NS_MAX_PARTS + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// X_0 = G / (|G| + eps), scaled, as hi + lo, 64 x 64 at a time; a tall G goes through LDS,
+__device__ __forceinline__ uint2 pack_fp8(const float (&v)[8]) {
+  int a = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
+  a = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], a, true);
+  int b = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
+  b = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], b, true);
+  return make_uint2((unsigned)a, (unsigned)b);
+}
+__device__ __forceinline__ void unpack_fp8(const uint2& q, float (&v)[8]) {
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.x, true);
+  const f32x2_t c = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.y, false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)q.y, true);
+  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
+}
+
+// X_0 = G / (|G| + eps), scaled, in two words, 64 x 64 at a time; a tall G goes through LDS,
 // so that it is read by rows and written by rows
 __global__ __launch_bounds__(256) void ns_ingest_kernel(NsSrc a, const double* __restrict__ part, int parts, double eps,
-                                                        f16* __restrict__ h, f16* __restrict__ lo, int sp, int lp,
+                                                        f16* __restrict__ h, uint8_t* __restrict__ lo, int sp, int lp,
                                                         int tall) {
   __shared__ float tile[64][65];
   __shared__ double red[4];
@@ -203,16 +221,17 @@ __global__ __launch_bounds__(256) void ns_ingest_kernel(NsSrc a, const double* _
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int q = tid + k * 256, y = q >> 3, x = (q & 7) * 8;
-    f16x8 hv, lv;
+    f16x8 hv;
+    float lv[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float f = (tall ? tile[y][x + e] : v[k][e]) * inv;
       hv[e] = (f16)f;
-      lv[e] = (f16)(f - (float)hv[e]);
+      lv[e] = (f - (float)hv[e]) * NS_SL;
     }
     const int64_t at = ((int64_t)b * sp + i0 + y) * lp + j0 + x;
     *reinterpret_cast<f16x8*>(h + at) = hv;
-    *reinterpret_cast<f16x8*>(lo + at) = lv;
+    *reinterpret_cast<uint2*>(lo + at) = pack_fp8(lv);
   }
 }
 
@@ -276,7 +295,7 @@ struct NsGemm {
   const f16* B; int64_t ldb, bsb;    // N x K, K contiguous (APPLY: K x N, N contiguous)
   int K, M, N, n;                    // of one matrix, whole tiles; n matrices
   f16* out; int64_t ldo, bso;        // D, P or the next X's high words
-  f16* lo;                           // APPLY: low words of X, in place
+  uint8_t* lo;                       // APPLY: X's second words, in place
   float* diag; int sp;               // rounding of D's diagonal
   float shift, c, mu;                // see the head of this file
   int last, tall;                    // APPLY: the result goes to dst
@@ -495,7 +514,8 @@ struct NsTile {
 #pragma unroll
     for (int part = 0; part < T / ER; ++part) {
       const int ip = i0 + part * ER;
-      f16x8 ga[NC], gb[NC];
+      f16x8 ga[NC];
+      uint2 gb[NC];
       bool ok[NC];
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -504,7 +524,7 @@ struct NsTile {
         if (MODE != NS_GRAM && ok[c]) {
           const int64_t at = b * g.bso + (int64_t)i * g.ldo + j;
           ga[c] = *reinterpret_cast<const f16x8*>((MODE == NS_SQUARE ? g.A : g.B) + at);
-          if (MODE == NS_APPLY) gb[c] = *reinterpret_cast<const f16x8*>(g.lo + at);
+          if (MODE == NS_APPLY) gb[c] = *reinterpret_cast<const uint2*>(g.lo + at);
         }
       }
       __syncthreads();
@@ -552,9 +572,11 @@ struct NsTile {
           }
         } else {
           const float sc = g.last ? 1.f / NS_SX : 1.f;
+          float l8[8];
+          unpack_fp8(gb[c], l8);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            x[e] = (g.mu * ((float)ga[c][e] + (float)gb[c][e]) + x[e] * (1.f / NS_SD)) * sc;
+            x[e] = (g.mu * __builtin_fmaf(l8[e], 1.f / NS_SL, (float)ga[c][e]) + x[e] * (1.f / NS_SD)) * sc;
         }
         if (turn) { t4[0] = (f32x4){x[0], x[1], x[2], x[3]}; t4[1] = (f32x4){x[4], x[5], x[6], x[7]}; }
         if (MODE == NS_APPLY && g.last) {
@@ -566,10 +588,10 @@ struct NsTile {
         for (int e = 0; e < 8; ++e) hv[e] = (f16)x[e];
         *reinterpret_cast<f16x8*>(g.out + at) = hv;
         if constexpr (MODE == NS_APPLY) {
-          f16x8 lv;
+          float lv[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) lv[e] = (f16)(x[e] - (float)hv[e]);
-          *reinterpret_cast<f16x8*>(g.lo + at) = lv;
+          for (int e = 0; e < 8; ++e) lv[e] = (x[e] - (float)hv[e]) * NS_SL;
+          *reinterpret_cast<uint2*>(g.lo + at) = pack_fp8(lv);
         }
       }
       if (turn) {      // 16 columns x 4 chunks of 8 rows per wave and pass

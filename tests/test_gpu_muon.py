@@ -53,7 +53,8 @@ def gradient(n, r, c, seed, decay=0.0):
 
 
 SHAPES = [(1, 1, 1), (1, 1, 7), (1, 5, 1), (2, 3, 3), (1, 16, 200), (1, 127, 129), (1, 128, 128), (2, 129, 64),
-          (3, 200, 333), (1, 517, 130), (2, 384, 128), (1, 1000, 300), (1, 640, 1291)]
+          (3, 200, 333), (1, 517, 130), (2, 384, 128), (1, 1000, 300), (1, 640, 1291), (3, 128, 512), (2, 512, 100), (2, 129, 512),
+          (1, 100, 513), (5, 33, 250), (2, 257, 17), (1, 129, 129)]
 
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
