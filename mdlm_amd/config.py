@@ -79,13 +79,19 @@ DEFAULTS = dict(
                 p_x0_dtype='bf16'),
   training=dict(ema=0.9999, antithetic_sampling=True,
                 importance_sampling=False, sampling_eps=1e-3,
-                change_of_variables=False),
+                change_of_variables=False,
+                # mdlm_amd extension: the training loss is NELBO - entropy_weight * mean
+                # entropy of the masked positions' predictions (0: the reference's loss)
+                entropy_weight=0.0),
   eval=dict(checkpoint_path='', disable_ema=False,
             compute_generative_perplexity=False, perplexity_batch_size=8,
             compute_perplexity_on_sanity=False,
             gen_ppl_eval_model_name_or_path='gpt2-large',
             generate_samples=True, num_batches=4),
-  optim=dict(weight_decay=0, lr=3e-4, beta1=0.9, beta2=0.999, eps=1e-8),
+  # name (mdlm_amd extension): adamw, as the reference, or muon -- the 2-D weights of the
+  # blocks' attention and MLP by orthogonalised momentum, everything else by AdamW
+  optim=dict(name='adamw', weight_decay=0, lr=3e-4, beta1=0.9, beta2=0.999, eps=1e-8,
+             momentum=0.95, ns_steps=5),
   trainer=dict(accelerator='cuda', num_nodes=1, devices=1, precision='bf16',
                accumulate_grad_batches=None, gradient_clip_val=1.0, max_steps=1_000_000,
                log_every_n_steps=10),

@@ -236,6 +236,23 @@ class Diffusion(_Base):
                                lse_skip_col=self.mask_index)
     return (logits, lse) if want_lse else logits
 
+  @torch.no_grad()
+  def score_tokens(self, x0, xt, sigma=None, top_k=0):
+    """Scores of the tokens x0 (B, L) where xt is masked, under the model's SUBS
+    prediction from xt: log-probability, entropy, log-sum-exp and the top_k
+    alternatives of every position (ops.SubsScores), without the (B, L, V)
+    table.  Known positions (xt not masked) score as the SUBS table does: 0 for
+    their own token.  sigma (B): needed with time_conditioning only."""
+    if x0.shape != xt.shape or xt.ndim != 2:
+      raise ValueError(f'score_tokens: x0 {tuple(x0.shape)} and xt {tuple(xt.shape)} must be (B, L) alike')
+    ops.check_token_ids(torch.stack([x0, xt]), self.vocab_size)
+    if sigma is None:
+      if self.time_conditioning:
+        raise ValueError('score_tokens: a time-conditioned model needs sigma')
+      sigma = torch.zeros(xt.shape[0], device=xt.device)
+    logits = self._backbone_logits(xt, sigma, masked_rows_only=True)
+    return ops.subs_scores(logits, xt, x0, self.mask_index, top_k=top_k)
+
   def forward(self, x, sigma):
     """Returns log score (diffusion.py:312-327): SUBS log-probs (B, L, V)."""
     ops.check_token_ids(x, self.vocab_size)

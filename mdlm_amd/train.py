@@ -91,7 +91,8 @@ class GradBuckets:
 
 class Trainer:
   def __init__(self, model, lr=None, betas=None, eps=None, weight_decay=None,
-               max_norm=1.0, num_warmup_steps=2500, dropout=None, group=None):
+               max_norm=1.0, num_warmup_steps=2500, dropout=None, group=None,
+               optimizer=None, entropy_weight=None):
     cfg = model.config
     bb = model.backbone
     dev = bb.vocab_embed.embedding.device
@@ -111,6 +112,14 @@ class Trainer:
     self.weight_decay = cfg.optim.weight_decay if weight_decay is None else weight_decay
     self.max_norm = max_norm
     self.num_warmup_steps = num_warmup_steps
+    self.optimizer = cfg.optim.get('name', 'adamw') if optimizer is None else optimizer
+    if self.optimizer not in ('adamw', 'muon'):
+      raise ValueError(f'Trainer: optimizer {self.optimizer!r} is neither adamw nor muon')
+    self.momentum = float(cfg.optim.get('momentum', 0.95))
+    self.ns_steps = int(cfg.optim.get('ns_steps', 5))
+    self.entropy_weight = float(cfg.training.get('entropy_weight', 0.0)
+                                if entropy_weight is None else entropy_weight)
+    self.last_entropy = None   # device scalar: mean entropy of the masked positions (entropy_weight != 0)
     self.p_drop = float(bb.blocks[0].dropout if dropout is None else dropout)
     self.ema_decay = float(cfg.training.ema)
     # Two counters, as in the reference: `step_count` is the optimizer's (Adam bias
@@ -169,6 +178,7 @@ class Trainer:
       slices.append(span(f'blocks.{i}.'))
     slices.append((0, span('blocks.0.')[0]))
     self.buckets = GradBuckets(self.G, slices, group)
+    self._split_parameters()
     self._ws = None
     self.A, self.micro = None, 0   # accumulation carry (allocated on first use)
     self.last_lr = None
@@ -177,6 +187,37 @@ class Trainer:
     self.last_grad_norm = None
 
   # ---------------------------------------------------------------- helpers
+  # weights whose update is orthogonalised (optimizer 'muon'): a stack per name, the
+  # blocks' copies lie at a constant stride in the flat buffers
+  MUON_NAMES = ('attn_qkv.weight', 'attn_out.weight', 'mlp.0.weight', 'mlp.2.weight')
+
+  def _split_parameters(self):
+    """The flat index ranges AdamW updates, and the stacks (offset, stride, rows, cols)
+    that are updated by orthogonalised momentum."""
+    self.adamw_ranges, self.muon_stacks = [(0, self.n_flat)], []
+    if self.optimizer != 'muon':
+      return
+    taken = []
+    for name in self.MUON_NAMES:
+      offs = [self.offsets[f'blocks.{i}.{name}'] for i in range(self.bb.n_blocks)]
+      (o, n, (r, c)), stride = offs[0], (offs[1][0] - offs[0][0] if len(offs) > 1 else offs[0][1])
+      assert all(e == (o + i * stride, n, (r, c)) for i, e in enumerate(offs))
+      self.muon_stacks.append((o, stride, r, c))
+      taken += [(e[0], e[0] + n) for e in offs]
+    self.adamw_ranges, at = [], 0
+    for a, b in sorted(taken):
+      if a > at:
+        self.adamw_ranges.append((at, a))
+      at = b
+    if at < self.n_flat:
+      self.adamw_ranges.append((at, self.n_flat))
+    nb = self.bb.n_blocks
+    self._muon_ws = torch.empty(max(ops.workspace_bytes('orthogonalize', nb, r, c) for _, _, r, c in self.muon_stacks),
+                                dtype=torch.uint8, device=self.dev)
+
+  def _stack(self, flat, o, stride, r, c):
+    return flat.as_strided((self.bb.n_blocks, r, c), (stride, c, 1), o)
+
   def _view(self, flat, name):
     o, n, shape = self.offsets[name]
     return flat[o:o + n].view(shape)
@@ -199,13 +240,16 @@ class Trainer:
     # rank 0's file and must get back ITS OWN stream (seed + rank), not rank 0's
     rank = mdist.env_rank()[0]
     return dict(P=self.P, M1=self.M1, M2=self.M2, E=self.E, step_count=self.step_count,
-                ema_updates=self.ema_updates,
+                ema_updates=self.ema_updates, optimizer=self.optimizer,
                 rng_seed=self.model._rng_seed - rank, rng_offset=self.model._rng_offset,
                 n_flat=self.n_flat)
 
   def load_state_dict(self, sd):
     if int(sd['n_flat']) != self.n_flat:
       raise ValueError(f"trainer state holds {sd['n_flat']} flat elements, model has {self.n_flat}")
+    if sd.get('optimizer', 'adamw') != self.optimizer:
+      raise ValueError(f"trainer state is of optimizer {sd.get('optimizer', 'adamw')!r}, this trainer's is "
+                       f'{self.optimizer!r}: its moments mean something else')
     self.P.copy_(sd['P']); self.M1.copy_(sd['M1']); self.M2.copy_(sd['M2'])
     if self.E is not None and sd.get('E') is not None:
       self.E.copy_(sd['E'])
@@ -378,7 +422,9 @@ class Trainer:
   def forward_backward(self, x0, attention_mask=None, t=None, u_xt=None,
                        accumulate=False, last=True):
     """Loss of one micro-batch and its gradients into the flat buffer G
-    (overwritten).  Returns (token_nll device scalar, nlls (B, L)).
+    (overwritten).  Returns (token_nll device scalar, nlls (B, L)); with
+    entropy_weight w the gradients are those of
+      token_nll - w * sum(entropy of the masked positions, attention-masked) / sum(attention_mask).
 
     Gradient accumulation (configs/config.yaml:68): micro-batches with
     `last=False` keep their gradients local (DDP no_sync) in a carry buffer;
@@ -476,8 +522,16 @@ class Trainer:
       ops.gemm_bf16(hfc, self._w16('output_layer.linear.weight'), lgc[:, :V], EPI_STORE,
                     bias=self._p32('output_layer.linear.bias'), ldc=lgc.stride(0))
       # ---- loss (diffusion.py:884-916) ----------------------------------------
-      nll_c = ops.subs_nll(lgc[:, :V], xt_c[:, None], x0_c[:, None], w_c,
-                           model.mask_index)
+      scores = None
+      if self.entropy_weight:
+        scores = ops.subs_scores(lgc[:, :V], xt_c, x0_c, model.mask_index)
+        nll_c = -scores.logp * w_c
+        ent_w = ((attention_mask.reshape(-1)[scc] * valid) / attention_mask.sum()).contiguous()
+        live = attention_mask.reshape(-1)[scc] * valid
+        self.last_entropy = (scores.entropy * live).sum() / live.sum().clamp(min=1)
+      else:
+        nll_c = ops.subs_nll(lgc[:, :V], xt_c[:, None], x0_c[:, None], w_c,
+                             model.mask_index)
       nlls.view(-1).index_add_(0, scc, nll_c.view(-1) * valid)
     sums = ops.nll_sums(nlls, attention_mask)
     token_nll = (sums[0] / sums[1]).float()
@@ -486,7 +540,12 @@ class Trainer:
     ws['d_md'].zero_()
     if n_pad:
       row_w = (w_c / attention_mask.sum()).contiguous()
-      ops.subs_nll_bwd(lgc[:, :V], xt_c, x0_c, row_w, dlc[:, :V], V, model.mask_index)
+      if scores is not None:
+        dlc[:, V:].zero_()     # the weight-gradient product reads the padding
+        ops.subs_scores_bwd(lgc[:, :V], xt_c, x0_c, model.mask_index, scores.lse, scores.entropy,
+                            g_logp=-row_w, g_entropy=-self.entropy_weight * ent_w, dlogits=dlc[:, :V])
+      else:
+        ops.subs_nll_bwd(lgc[:, :V], xt_c, x0_c, row_w, dlc[:, :V], V, model.mask_index)
       # logits = hf Wv^T + bv (rows of dWv beyond V stay in the split-K partials)
       self._weight_grad(dlc, hfc, self._g('output_layer.linear.weight'), ws['bias_v'], ws)
       self._g('output_layer.linear.bias').copy_(ws['bias_v'][:V])
@@ -564,7 +623,9 @@ class Trainer:
   # ----------------------------------------------------------------- optimizer
   def optimizer_step(self):
     """clip_grad_norm_ + AdamW + lr schedule + EMA (diffusion.py:254-259,
-    449-471) and the bf16 refresh of the GEMM weights, one launch."""
+    449-471) and the bf16 refresh of the GEMM weights, one launch.  Optimizer
+    'muon': the blocks' stacks of 2-D weights by orthogonalised momentum (M1 holds
+    it), the ranges between them by AdamW; one gradient norm clips both."""
     self.buckets.wait_all()
     lr = constant_warmup_lr(self.lr, self.step_count, self.num_warmup_steps)
     self.step_count += 1
@@ -578,9 +639,17 @@ class Trainer:
       self.ema_updates += 1
       ne = self.ema_updates
       omd = 1.0 - min(self.ema_decay, (1 + ne) / (10 + ne))
-    ops.adamw_ema(self.P, self.G, self.M1, self.M2, self.E, self.W16, lr, self.betas[0],
-                  self.betas[1], self.eps, self.weight_decay, n, omd, sumsq=self._sumsq,
-                  max_norm=self.max_norm or 0.0, grad_scale=scale)
+    part = lambda flat, a, b: None if flat is None else flat[a:b]
+    for a, b in self.adamw_ranges:
+      ops.adamw_ema(self.P[a:b], self.G[a:b], self.M1[a:b], self.M2[a:b], part(self.E, a, b), self.W16[a:b], lr,
+                    self.betas[0], self.betas[1], self.eps, self.weight_decay, n, omd, sumsq=self._sumsq,
+                    max_norm=self.max_norm or 0.0, grad_scale=scale)
+    for s in self.muon_stacks:
+      ops.muon_update(self._stack(self.P, *s), self._stack(self.G, *s), self._stack(self.M1, *s), lr,
+                      ema=None if self.E is None else self._stack(self.E, *s), w16=self._stack(self.W16, *s),
+                      momentum=self.momentum, weight_decay=self.weight_decay, steps=self.ns_steps,
+                      sumsq=self._sumsq, max_norm=self.max_norm or 0.0, grad_scale=scale,
+                      ema_one_minus_decay=omd, ws=self._muon_ws)
     if getattr(self.model, 'ema', None) is not None:
       self.model.ema.num_updates = self.ema_updates
     self.bb.refresh()

@@ -108,3 +108,42 @@ def test_wrappers_refuse_cpu_tensors():
                lambda: ops.orthogonalize(x), lambda: ops.muon_update(x, x, x, 1e-3)):
     with pytest.raises(RuntimeError, match='no CPU fallback'):
       call()
+
+
+def test_config_keys():
+  from mdlm_amd.config import load_config
+  cfg = load_config([])
+  assert cfg.optim.name == 'adamw' and cfg.training.entropy_weight == 0.0
+  cfg = load_config(['optim.name=muon', 'optim.momentum=0.9', 'training.entropy_weight=0.1'])
+  assert cfg.optim.name == 'muon' and cfg.optim.momentum == 0.9 and cfg.training.entropy_weight == 0.1
+
+
+def test_muon_stacks_cover_the_blocks():
+  """The flat layout that the optimizer splits: stacks at a constant stride, AdamW's
+  ranges and the stacks together every element once."""
+  from types import SimpleNamespace
+
+  from mdlm_amd.shadow import flat_layout
+  from mdlm_amd.train import Trainer
+  shapes = {'vocab_embed.embedding': (30, 16)}
+  for i in range(3):
+    shapes.update({f'blocks.{i}.norm1.weight': (16,), f'blocks.{i}.attn_qkv.weight': (48, 16),
+                   f'blocks.{i}.attn_out.weight': (16, 16), f'blocks.{i}.norm2.weight': (16,),
+                   f'blocks.{i}.mlp.0.weight': (64, 16), f'blocks.{i}.mlp.0.bias': (64,),
+                   f'blocks.{i}.mlp.2.weight': (16, 64), f'blocks.{i}.mlp.2.bias': (16,),
+                   f'blocks.{i}.adaLN_modulation.weight': (96, 8)})
+  shapes['output_layer.linear.weight'] = (30, 16)
+  table, n_flat = flat_layout(list(shapes.values()))
+  t = SimpleNamespace(optimizer='muon', n_flat=n_flat, offsets=dict(zip(shapes, table)), bb=SimpleNamespace(n_blocks=3),
+                      MUON_NAMES=Trainer.MUON_NAMES, dev='cpu')
+  Trainer._split_parameters(t)
+  seen = torch.zeros(n_flat, dtype=torch.int32)
+  for a, b in t.adamw_ranges:
+    seen[a:b] += 1
+  for s in t.muon_stacks:
+    Trainer._stack(t, seen, *s).add_(1)
+  assert (seen == 1).all()
+  assert len(t.muon_stacks) == 4 and len(t.adamw_ranges) == 3 * 3 + 1
+  t.optimizer = 'adamw'
+  Trainer._split_parameters(t)
+  assert t.adamw_ranges == [(0, n_flat)] and t.muon_stacks == []
