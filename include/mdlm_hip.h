@@ -555,7 +555,7 @@ int mdlm_subs_scores_bwd(const void* logits, int64_t ld, int dtype,
  * go towards 1, singular vectors stay.  No reference counterpart (its optimizer
  * is AdamW, diffusion.py:449-459).  n matrices (rows, cols), fp32 or bf16, rows
  * `ld` and matrices `stride` elements apart; out bf16 (the products round their
- * operands to fp16: the result is good to bf16).  c != 0, |b / 2c| <= 8.
+ * operands to fp16: the result is good to bf16).  |a| <= 16, 0 < |c| <= 32, |b^2 / 4c| <= 16.
  * ws: mdlm_orthogonalize_workspace_bytes(n, rows, cols), 256-byte aligned. */
 int mdlm_orthogonalize(const void* g, int64_t ldg, int64_t g_stride, int dtype,
                        void* out_bf16, int64_t ldo, int64_t out_stride, int n,

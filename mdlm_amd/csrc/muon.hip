@@ -738,8 +738,9 @@ static int ns_check(const char* who, int n, int rows, int cols, int64_t ld, int6
   MDLM_CHECK_ARG((rows < cols ? rows : cols) <= (1 << 15), "%s: the smaller side must be at most 32768", who);
   MDLM_CHECK_ARG(ld >= cols && (n == 1 || bs >= (int64_t)(rows - 1) * ld + cols), "%s: overlapping rows or matrices", who);
   MDLM_CHECK_ARG(steps >= 1 && steps <= 32, "%s: steps=%d is outside 1..32", who, steps);
-  MDLM_CHECK_ARG(isfinite(a) && isfinite(b) && isfinite(c) && fabs(a) <= 16 && c != 0.0 && fabs(b / (2 * c)) <= 8 &&
-                   fabs(c) <= 16,
+  // the completed square's constant is what rounding D costs: 2.8 for the usual coefficients
+  MDLM_CHECK_ARG(isfinite(a) && isfinite(b) && isfinite(c) && fabs(a) <= 16 && c != 0.0 && fabs(c) <= 32 &&
+                   fabs(b * b / (4 * c)) <= 16,
                  "%s: coefficients (%g, %g, %g) are outside what the fp16 products hold", who, a, b, c);
   MDLM_CHECK_ARG(eps > 0.0 && isfinite(eps), "%s: eps must be positive", who);
   return 0;

@@ -16,7 +16,11 @@ constexpr float SC_L2E = 1.4426950408889634f;
 constexpr float SC_LN2 = 0.6931471805599453f;
 constexpr float SC_NEG = -1000000.f;      // Diffusion.neg_infinity
 constexpr int SC_MAX_K = 64;
-constexpr int64_t SC_WIDE_ROWS = 512;
+// Up to so many rows a workgroup has a CU to itself and its latency counts: 1024 threads, if
+// the row has a chunk for each.  Measured, us (256 / 1024 threads, bf16, 50258 columns): 64 rows with
+// 8 alternatives 20 / 16, 1024 rows 32 / 44; gradient of 64 rows of 128000 columns 26 / 14.
+constexpr int64_t SC_WIDE_ROWS = 256;
+constexpr int SC_WIDE_BYTES = 16 * 1024;
 
 // order of the alternatives: larger logit first (NaN above all, -0 = +0), then
 // the lower index; unique per column, 0 for none
@@ -100,12 +104,16 @@ template <> __device__ __forceinline__ void unpack16<bf16_t, float[8]>(const uin
 constexpr float SC_FLOOR = -1e30f;
 struct Running {
   float m = SC_FLOOR, m2 = SC_FLOOR * SC_L2E, s = 0.f, s1 = 0.f;
+  float next = SC_FLOOR;        // the largest maximum of any other chunk than `best`, which holds m
+  int best = -1;
   template <int N>
-  __device__ __forceinline__ void add(const float (&f)[N]) {
+  __device__ __forceinline__ void add(const float (&f)[N], int chunk) {
     float mx = f[0];
 #pragma unroll
     for (int k = 1; k < N; ++k) mx = fmaxf(mx, f[k]);
+    next = fmaxf(next, fminf(m, mx));
     if (mx > m) {
+      best = chunk;
       const float n2 = mx * SC_L2E, d = m2 - n2, sc = __builtin_amdgcn_exp2f(d);
       s1 = __builtin_fmaf(d, s, s1) * sc;
       s *= sc;
@@ -202,9 +210,9 @@ __device__ void slow_top(const T* row, int V, int mask, int k, float m, float lz
 //
 // Alternatives: the maxima of 64 groups of threads are at hand after the pass; the
 // k-th largest of them, tau, is a lower bound of the k-th best logit (k groups
-// reach it).  Only threads whose own maximum reaches tau look at their share
-// again (from the caches), a handful of columns pass, and each one's rank among
-// them is its place.  Ranks go by (logit, index) keys: the order in which the
+// reach it).  Only threads whose own maximum reaches tau look again (from the
+// caches), at the one chunk that holds it unless another's maximum reaches tau
+// too; a handful of columns pass, and each one's rank among them is its place.  Ranks go by (logit, index) keys: the order in which the
 // atomic hands out list places does not show.
 template <typename T, int BLOCK>
 __global__ __launch_bounds__(BLOCK) void subs_scores_kernel(
@@ -236,7 +244,7 @@ __global__ __launch_bounds__(BLOCK) void subs_scores_kernel(
 #pragma unroll
       for (int e = 0; e < E; ++e) if (e == sp.mask_elem) f[e] = -INFINITY;
     }
-    run.add(f);
+    run.add(f, i);
   };
   for (int i = tid; i < sp.n; i += U * BLOCK) {
     uint4 q[U];
@@ -248,7 +256,7 @@ __global__ __launch_bounds__(BLOCK) void subs_scores_kernel(
   const int alone = tid < sp.head + sp.tail ? sp.single(tid) : -1;
   if (alone >= 0 && alone != mask) {
     const float f[1] = {elem<T>::load(row + alone)};
-    run.add(f);
+    run.add(f, -1);
   }
   // ---- across the workgroup
   const float own = run.m;
@@ -311,13 +319,22 @@ __global__ __launch_bounds__(BLOCK) void subs_scores_kernel(
           if (at < ScoreShared<BLOCK>::CAP) sh.cand[at] = score_key(x, v);
         }
       };
-      for (int c = tid; c < sp.n; c += BLOCK) {
-        float f[E];
-        unpack16<T>(chunks[c], f);
+      const bool all = run.next >= tau;
+      if (all || run.best < 0) { if (alone >= 0) offer(elem<T>::load(row + alone), alone); }
+      const int last = all ? sp.n : run.best + 1;
+      for (int c0 = all ? tid : run.best; c0 >= 0 && c0 < last; c0 += 8 * BLOCK) {
+        uint4 q[8];
 #pragma unroll
-        for (int e = 0; e < E; ++e) offer(f[e], sp.head + c * E + e);
+        for (int u = 0; u < 8; ++u) if (c0 + u * BLOCK < last) q[u] = chunks[c0 + u * BLOCK];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (c0 + u * BLOCK < last) {
+            float f[E];
+            unpack16<T>(q[u], f);
+#pragma unroll
+            for (int e = 0; e < E; ++e) offer(f[e], sp.head + (c0 + u * BLOCK) * E + e);
+          }
       }
-      if (alone >= 0) offer(elem<T>::load(row + alone), alone);
     }
     __syncthreads();
     n = sh.count;
@@ -466,10 +483,9 @@ extern "C" int mdlm_subs_scores(const void* logits, int64_t ld, int dtype, const
                  "subs_scores: top_k=%d must be at most %d and less than V=%d", top_k, SC_MAX_K, V);
   MDLM_CHECK_ARG(top_k == 0 || (top_logp && top_ids), "subs_scores: null pointer (alternatives)");
   (void)ws;
-  // Few rows leave CUs idle: a row's latency counts, so a workgroup of 1024.
 #define SC_LAUNCH(T, B) \
   subs_scores_kernel<T, B><<<(unsigned)rows, B, 0, (hipStream_t)stream>>>((const T*)logits, ld, xt, x0, logp, entropy, lse, top_logp, top_ids, V, mask_index, top_k)
-  const bool wide = rows <= SC_WIDE_ROWS;
+  const bool wide = rows <= SC_WIDE_ROWS && (int64_t)V * (dtype == MDLM_BF16 ? 2 : 4) >= SC_WIDE_BYTES;
   if (dtype == MDLM_BF16) { if (wide) SC_LAUNCH(bf16_t, 1024); else SC_LAUNCH(bf16_t, 256); }
   else if (dtype == MDLM_F32) { if (wide) SC_LAUNCH(float, 1024); else SC_LAUNCH(float, 256); }
 #undef SC_LAUNCH
@@ -491,7 +507,7 @@ extern "C" int mdlm_subs_scores_bwd(const void* logits, int64_t ld, int dtype, c
   MDLM_CHECK_ARG(top_k == 0 || (top_ids && g_top), "subs_scores_bwd: null pointer (alternatives)");
 #define SC_LAUNCH(T, B) \
   subs_scores_bwd_kernel<T, B><<<(unsigned)rows, B, 0, (hipStream_t)stream>>>((const T*)logits, ld, xt, x0, lse, entropy, g_logp, g_entropy, top_ids, g_top, top_k, (T*)dlogits, ldo, V, mask_index)
-  const bool wide = rows <= SC_WIDE_ROWS;
+  const bool wide = rows <= SC_WIDE_ROWS && (int64_t)V * (dtype == MDLM_BF16 ? 2 : 4) >= SC_WIDE_BYTES;
   if (dtype == MDLM_BF16) { if (wide) SC_LAUNCH(bf16_t, 1024); else SC_LAUNCH(bf16_t, 256); }
   else if (dtype == MDLM_F32) { if (wide) SC_LAUNCH(float, 1024); else SC_LAUNCH(float, 256); }
 #undef SC_LAUNCH
