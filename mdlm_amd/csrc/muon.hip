@@ -509,8 +509,7 @@ struct NsTile {
     float* const tile = reinterpret_cast<float*>(smem);
     // the other side of a symmetric product, or a tall matrix's own orientation
     const bool turn = MODE == NS_APPLY ? g.last && g.tall : tm != tn;
-    constexpr int CH = T / 8, NC = ER * CH / THREADS > 0 ? ER * CH / THREADS : 1;      // chunks of 8: per row, per thread
-    static_assert(NC * THREADS == ER * CH || ER * CH < THREADS, "whole chunks per thread");
+    constexpr int CH = T / 8, NC = (ER * CH + THREADS - 1) / THREADS;      // chunks of 8: per row, per thread
 #pragma unroll
     for (int part = 0; part < T / ER; ++part) {
       const int ip = i0 + part * ER;
@@ -666,6 +665,9 @@ static int ns_launch(const NsGemm& g, hipStream_t st) {
 //   A of 768 x 768:            64: 6.2 / 8.9 (deep / shallow)   128: 13
 //   A of 1024 x 4096:          64: 16 / 30                      128: 41
 //   A of 2048 x 2048:          64: 22 / 19                      128: 25
+// For the symmetric products 96 x 96 tiles are in between, where all of them are resident
+// at once (two workgroups per CU) and not too few to fill it (64 shallow / 96 / 128):
+//   A of 12 x 768 x 2304: 31 / 28 / 30   A of 6 x 768 x 2304: 20 / 18 / 28   A of 2 x 2048 x 8192: 140 / 86 / 106
 // With more, the rounds of tiles that a CU goes through, times what a slab of one
 // costs with the chip full (us, measured on 4096 x 4096: 128: 0.59 in pairs, 192:
 // 1.16, 256: 1.5; P X: 128: 0.54, 256: 2.0):
@@ -676,6 +678,10 @@ static int ns_launch(const NsGemm& g, hipStream_t st) {
 template <int MODE>
 static int ns_gemm(const NsGemm& g, int cus, hipStream_t st) {
   const int64_t t128 = ns_tiles(MODE, g, 128);
+  if constexpr (MODE != NS_APPLY) {
+    const int64_t t96 = ns_tiles(MODE, g, 96);
+    if (t96 * 5 >= cus * 4 && t96 <= 2 * cus) return ns_launch<MODE, 96, 2, 2, 3>(g, st);
+  }
   if (t128 <= cus)
     return ns_tiles(MODE, g, 64) <= 2 * cus ? ns_launch<MODE, 64, 2, 2, 4>(g, st) : ns_launch<MODE, 64, 2, 2, 2>(g, st);
   auto rounds = [&](int T, int slots) { return (double)((ns_tiles(MODE, g, T) + slots - 1) / slots); };
