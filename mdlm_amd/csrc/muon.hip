@@ -93,56 +93,68 @@ __device__ __forceinline__ float clip_coef(const NsSrc& a) {
   }
   return coef;
 }
-// eight columns of row r of matrix b, from column c (a multiple of 8) on; 0 past the last.
-// STEP: the momentum is moved first (the one pass that does so comes before the others).
-template <bool STEP>
-__device__ __forceinline__ void src_load8(const NsSrc& a, int b, int r, int c, float coef, float (&v)[8]) {
+// eight columns of row r of matrix b, from column c (a multiple of 8) on; 0 past the last
+struct NsRaw { float g[8], m[8]; };
+__device__ __forceinline__ void src_fetch8(const NsSrc& a, int b, int r, int c, NsRaw& w) {
   const int64_t at = b * a.bs + r * a.ld + c;
-  float g[8], m[8];
   if (a.vec && c + 8 <= a.cols) {
     if (a.bf16) {
       const uint4 q = *reinterpret_cast<const uint4*>((const bf16_t*)a.g + at);
       const unsigned u[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) g[e] = __uint_as_float(e & 1 ? u[e >> 1] & 0xffff0000u : u[e >> 1] << 16);
+      for (int e = 0; e < 8; ++e) w.g[e] = __uint_as_float(e & 1 ? u[e >> 1] & 0xffff0000u : u[e >> 1] << 16);
     } else {
-      const float4 x = *reinterpret_cast<const float4*>((const float*)a.g + at);
-      const float4 y = *reinterpret_cast<const float4*>((const float*)a.g + at + 4);
-      g[0] = x.x; g[1] = x.y; g[2] = x.z; g[3] = x.w; g[4] = y.x; g[5] = y.y; g[6] = y.z; g[7] = y.w;
+      const f32x4 x = *reinterpret_cast<const f32x4*>((const float*)a.g + at);
+      const f32x4 y = *reinterpret_cast<const f32x4*>((const float*)a.g + at + 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w.g[e] = e < 4 ? x[e & 3] : y[e & 3];
     }
     if (a.m) {
-      const float4 x = *reinterpret_cast<const float4*>(a.m + at), y = *reinterpret_cast<const float4*>(a.m + at + 4);
-      m[0] = x.x; m[1] = x.y; m[2] = x.z; m[3] = x.w; m[4] = y.x; m[5] = y.y; m[6] = y.z; m[7] = y.w;
+      const f32x4 x = *reinterpret_cast<const f32x4*>(a.m + at), y = *reinterpret_cast<const f32x4*>(a.m + at + 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w.m[e] = e < 4 ? x[e & 3] : y[e & 3];
     }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const bool in = c + e < a.cols;
-      g[e] = !in ? 0.f : a.bf16 ? bf16_to_f32(((const bf16_t*)a.g)[at + e]) : ((const float*)a.g)[at + e];
-      m[e] = in && a.m ? a.m[at + e] : 0.f;
+      w.g[e] = !in ? 0.f : a.bf16 ? bf16_to_f32(((const bf16_t*)a.g)[at + e]) : ((const float*)a.g)[at + e];
+      w.m[e] = in && a.m ? a.m[at + e] : 0.f;
     }
   }
+}
+// what is orthogonalised, from what was fetched.  STEP: the momentum is moved first (the
+// one pass that does so comes before the others).
+template <bool STEP>
+__device__ __forceinline__ void src_finish8(const NsSrc& a, int b, int r, int c, float coef, NsRaw& w, float (&v)[8]) {
   if (!a.m) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = g[e];
+    for (int e = 0; e < 8; ++e) v[e] = w.g[e];
     return;
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    g[e] *= coef;
-    if (STEP) m[e] = m[e] + (g[e] - m[e]) * (1.f - a.momentum);
-    v[e] = g[e] + a.momentum * (m[e] - g[e]);
+    const float g = w.g[e] * coef;
+    if (STEP) w.m[e] = w.m[e] + (g - w.m[e]) * (1.f - a.momentum);
+    v[e] = g + a.momentum * (w.m[e] - g);
   }
   if (STEP) {
+    const int64_t at = b * a.bs + r * a.ld + c;
     if (a.vec && c + 8 <= a.cols) {
-      *reinterpret_cast<float4*>(a.m + at) = make_float4(m[0], m[1], m[2], m[3]);
-      *reinterpret_cast<float4*>(a.m + at + 4) = make_float4(m[4], m[5], m[6], m[7]);
+      *reinterpret_cast<f32x4*>(a.m + at) = (f32x4){w.m[0], w.m[1], w.m[2], w.m[3]};
+      *reinterpret_cast<f32x4*>(a.m + at + 4) = (f32x4){w.m[4], w.m[5], w.m[6], w.m[7]};
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (c + e < a.cols) a.m[at + e] = m[e];
+        if (c + e < a.cols) a.m[at + e] = w.m[e];
     }
   }
+}
+template <bool STEP>
+__device__ __forceinline__ void src_load8(const NsSrc& a, int b, int r, int c, float coef, float (&v)[8]) {
+  NsRaw w;
+  src_fetch8(a, b, r, c, w);
+  src_finish8<STEP>(a, b, r, c, coef, w, v);
 }
 
 // momentum (in place) and the partial sums of squares of what will be orthogonalised,
@@ -153,14 +165,26 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsSrc a, double* __restric
   const float coef = a.m ? clip_coef(a) : 1.f;
   const unsigned per_row = (a.cols + 7) / 8, chunks = per_row * a.rows, step = gridDim.x * 256;
   double acc = 0.0;
-  for (unsigned q = blockIdx.x * 256 + threadIdx.x; q < chunks; q += step) {
-    const unsigned r = q / per_row;
-    float v[8];
-    src_load8<true>(a, b, r, (q - r * per_row) * 8, coef, v);
-    double s = 0.0;
+  // U chunks are fetched before the first is finished: a store in between would hold up the next load
+  constexpr int U = 2;
+  for (unsigned q0 = blockIdx.x * 256 + threadIdx.x; q0 < chunks; q0 += U * step) {
+    NsRaw raw[U];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s += (double)v[e] * (double)v[e];
-    acc += s;
+    for (int u = 0; u < U; ++u) {
+      const unsigned q = q0 + u * step, r = q / per_row;
+      if (q < chunks) src_fetch8(a, b, r, (q - r * per_row) * 8, raw[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned q = q0 + u * step, r = q / per_row;
+      if (q >= chunks) continue;
+      float v[8];
+      src_finish8<true>(a, b, r, (q - r * per_row) * 8, coef, raw[u], v);
+      double s = 0.0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += (double)v[e] * (double)v[e];
+      acc += s;
+    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) acc += __shfl_xor(acc, o);
