@@ -293,7 +293,11 @@ __global__ __launch_bounds__(BLOCK) void subs_scores_kernel(
   if (tid == 0) {
     lse[r] = m + lz;
     ent[r] = (l2s - s1 / s) * SC_LN2;
-    logp[r] = tgt < 0 || tgt >= V ? 0.f : tgt == mask ? (xtgt + SC_NEG) - (m + lz) : (xtgt - m) - lz;
+    // a row without a finite logit has no scores, not even the mask token's
+    logp[r] = tgt < 0 || tgt >= V ? 0.f
+              : m == -INFINITY   ? NAN
+              : tgt == mask      ? (xtgt + SC_NEG) - (m + lz)
+                                 : (xtgt - m) - lz;
   }
   if (k == 0) return;
   float* tl = top_logp + r * k;

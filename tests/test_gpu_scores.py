@@ -165,6 +165,21 @@ def test_scores_of_every_kind_of_row(ops, dtype):
   assert s.lse[1] == -math.inf and s.lse[12] == -math.inf
 
 
+def test_scores_of_one_column_and_of_the_mask_token(ops):
+  """V = 1 is the mask column alone: a masked position has no distribution; in a row
+  that has one, the mask token scores its logit - 1e6 - lse."""
+  x = torch.zeros(2, 1, device='cuda')
+  s = ops.subs_scores(x, torch.tensor([0, 5], device='cuda'), torch.tensor([0, 5], device='cuda'), 0)
+  assert s.logp[0].isnan() and s.entropy[0].isnan() and s.lse[0] == -math.inf
+  assert s.logp[1] == 0 and s.entropy[1] == 0
+  V, mask = 50, 3
+  x = make_logits(2, V, torch.float32, 'tight', seed=1)
+  x[1] = -math.inf
+  s = ops.subs_scores(x, torch.full((2,), mask, device='cuda'), torch.full((2,), mask, device='cuda'), mask, top_k=49)
+  assert abs(s.logp[0].item() - (x[0, mask].item() + NEG - s.lse[0].item())) <= 1
+  assert s.logp[1].isnan() and (s.top_ids != mask).all()
+
+
 def test_scores_targets_that_are_no_tokens(ops):
   V, mask = 300, 299
   x = make_logits(4, V, torch.float32, 'tight', seed=9)
