@@ -556,7 +556,9 @@ int mdlm_subs_scores_bwd(const void* logits, int64_t ld, int dtype,
  * is AdamW, diffusion.py:449-459).  n matrices (rows, cols), fp32 or bf16, rows
  * `ld` and matrices `stride` elements apart; out bf16 (the products round their
  * operands to fp16: the result is good to bf16).  |a| <= 16, 0 < |c| <= 32, |b^2 / 4c| <= 16.
- * ws: mdlm_orthogonalize_workspace_bytes(n, rows, cols), 256-byte aligned. */
+ * `out` may be g itself.  ws: mdlm_orthogonalize_workspace_bytes(n, rows, cols),
+ * 256-byte aligned; calls that overlap in time (two streams, two captured graphs
+ * replayed at once) need one each. */
 int mdlm_orthogonalize(const void* g, int64_t ldg, int64_t g_stride, int dtype,
                        void* out_bf16, int64_t ldo, int64_t out_stride, int n,
                        int rows, int cols, int steps, double a, double b,
@@ -571,7 +573,7 @@ int mdlm_orthogonalize(const void* g, int64_t ldg, int64_t g_stride, int dtype,
  *   p <- p (1 - lr weight_decay) - lr update_scale O
  * p, g, m, ema (may be NULL): fp32, w_bf16 (may be NULL): bf16, all of the same
  * layout (rows `ld`, matrices `stride` elements apart).  g is not written.
- * ws: mdlm_orthogonalize_workspace_bytes(n, rows, cols), 256-byte aligned. */
+ * The buffers must not overlap.  ws: as mdlm_orthogonalize. */
 int mdlm_muon_update(float* p, const float* g, float* m, float* ema,
                      void* w_bf16, int64_t ld, int64_t stride, int n, int rows,
                      int cols, float lr, float momentum, float weight_decay,

@@ -809,6 +809,9 @@ extern "C" int mdlm_muon_update(float* p, const float* g, float* m, float* ema, 
   if (n == 0 || rows == 0 || cols == 0) return 0;
   MDLM_CHECK_ARG(p && g && m && ws, "muon_update: null pointer");
   if (int rc = ns_check("muon_update", n, rows, cols, ld, stride, steps, a, b, c, eps)) return rc;
+  MDLM_CHECK_ARG(p != g && p != m && g != m && ema != p && ema != m && (!ema || ema != g) && w_bf16 != (void*)p &&
+                   w_bf16 != (void*)m && (!w_bf16 || (w_bf16 != (void*)ema && w_bf16 != (const void*)g)),
+                 "muon_update: the buffers must be different ones");
   MDLM_CHECK_ARG(momentum >= 0.f && momentum < 1.f, "muon_update: momentum %g is outside [0, 1)", momentum);
   MDLM_CHECK_ARG(((uintptr_t)ws & 255) == 0, "muon_update: the workspace must be 256-byte aligned");
   NsSrc src = {};

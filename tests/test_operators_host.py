@@ -62,7 +62,7 @@ def test_orthogonalize_refusals(bad, text):
 
 
 def _muon(**kw):
-  a = dict(p=256, g=256, m=256, ema=0, w=0, ld=64, stride=4096, n=2, rows=64, cols=64, lr=1e-3, momentum=0.95, wd=0.0,
+  a = dict(p=256, g=512, m=768, ema=0, w=0, ld=64, stride=4096, n=2, rows=64, cols=64, lr=1e-3, momentum=0.95, wd=0.0,
            scale=1.0, steps=5, a=3.4445, b=-4.775, c=2.0315, eps=1e-7, omd=0.0, sumsq=0, max_norm=0.0, gs=1.0, ws=256,
            st=0)
   a.update(kw)
@@ -72,7 +72,10 @@ def _muon(**kw):
 @pytest.mark.parametrize('bad,text', [
   (dict(p=0), 'null pointer'), (dict(m=0), 'null pointer'), (dict(ws=0), 'null pointer'), (dict(ld=60), 'overlapping'),
   (dict(stride=100), 'overlapping'), (dict(momentum=1.0), 'momentum'), (dict(momentum=-0.1), 'momentum'),
-  (dict(momentum=math.nan), 'momentum'), (dict(steps=0), 'steps'), (dict(ws=16), 'aligned')])
+  (dict(momentum=math.nan), 'momentum'), (dict(steps=0), 'steps'), (dict(ws=16), 'aligned'),
+  (dict(g=256), 'different'), (dict(m=256), 'different'), (dict(m=512), 'different'), (dict(ema=256), 'different'),
+  (dict(ema=768), 'different'), (dict(ema=512), 'different'), (dict(w=256), 'different'), (dict(w=512), 'different'),
+  (dict(ema=1024, w=1024), 'different')])
 def test_muon_update_refusals(bad, text):
   with pytest.raises(RuntimeError, match=text):
     _muon(**bad)
