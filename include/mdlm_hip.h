@@ -522,7 +522,7 @@ int mdlm_adamw_ema(float* p, const float* g, float* m, float* v, float* ema,
  *     mask column excluded, best first, equal logits by index (NaN counts as
  *     largest), and their l.  0 <= top_k <= 64, top_k < V; 0: not computed.
  * A row with xt != mask_index is known and not read: logp is 0 for x0 == xt and
- * -1e6 otherwise, entropy and lse are 0, the alternatives are xt (0) and the lowest
+ * -1e6 for another token, entropy and lse are 0, the alternatives are xt (0) and the lowest
  * other indices (-1e6).  A masked row without a finite logit, or with a NaN or
  * +inf outside the mask column, has no distribution: its scores are NaN (lse -inf
  * where every logit is -inf).

@@ -41,12 +41,13 @@ __device__ __forceinline__ unsigned long long wave_max_u64(unsigned long long v)
   return v;
 }
 
-// A position that is not masked: log-probability 0 for its own token, -1e6 for
-// every other one; the alternatives are its token and the lowest other ids.
+// A position that is not masked: log-probability 0 for its own token (and for what is
+// no token), -1e6 for every other one; the alternatives are its token and the lowest other ids.
 __device__ __forceinline__ void known_row(int64_t r, int64_t tok, const int64_t* x0, float* logp, float* ent, float* lse,
                                           float* top_logp, int64_t* top_ids, int V, int mask, int k, int tid) {
   if (tid == 0) {
-    logp[r] = x0[r] == tok ? 0.f : SC_NEG;
+    const int64_t tgt = x0[r];
+    logp[r] = tgt == tok || tgt < 0 || tgt >= V ? 0.f : SC_NEG;
     ent[r] = 0.f;
     lse[r] = 0.f;
   }

@@ -76,7 +76,7 @@ def oracle(logits, xt, x0, mask, k):
     t = int(xt[r])
     if t == mask:
       continue
-    logp[r] = 0.0 if int(x0[r]) == t else NEG
+    logp[r] = 0.0 if int(x0[r]) == t or not ok[r] else NEG
     ent[r] = lse[r] = 0.0
     if k:
       ids[r] = torch.tensor(([t] + [v for v in range(V) if v not in (t, mask)])[:k])
@@ -185,6 +185,8 @@ def test_scores_targets_that_are_no_tokens(ops):
   x = make_logits(4, V, torch.float32, 'tight', seed=9)
   xt = torch.full((4,), mask)
   s = check(ops, x, xt, torch.tensor([-1, V, -100, 2 ** 40]), mask, 3)
+  assert (s.logp == 0).all()
+  s = check(ops, x, torch.tensor([mask, 7, 0, mask]), torch.tensor([-100, -100, V, 2 ** 40]), mask, 3)   # known rows too
   assert (s.logp == 0).all()
 
 
