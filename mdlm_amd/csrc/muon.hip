@@ -232,7 +232,9 @@ __global__ __launch_bounds__(256) void ns_ingest_kernel(NsSrc a, const double* _
   for (int o = 32; o > 0; o >>= 1) t += __shfl_xor(t, o);
   if ((tid & 63) == 0) red[tid >> 6] = t;
   __syncthreads();
-  const float inv = (float)((double)NS_SX / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + eps));
+  // finite, so that an all-zero matrix stays zero whatever eps (NaN stays NaN)
+  const double scale = (double)NS_SX / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + eps);
+  const float inv = scale > 3.4e38 ? 3.4e38f : (float)scale;
   if (tall) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {

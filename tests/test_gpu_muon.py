@@ -113,6 +113,8 @@ def test_orthogonalize_zero_tiny_huge_and_bad(ops):
     assert rel(o[i], want[k]) < tol_factor(5) + 2.0 ** -8
   tiny = gradient(1, 40, 40, seed=6) * 1e-25  # squares below the fp32 range
   assert rel(ops.orthogonalize(tiny.cuda(), eps=1e-40), oracle(tiny, eps=1e-40)) < tol_factor(5) + 2.0 ** -8
+  for eps in (1e-40, 1e-300):
+    assert (ops.orthogonalize(torch.zeros(70, 20, device='cuda'), eps=eps) == 0).all()
 
 
 def test_orthogonalize_strides_out_and_workspace(ops):
