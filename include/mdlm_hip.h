@@ -541,7 +541,8 @@ int mdlm_subs_scores(const void* logits, int64_t ld, int dtype,
  * zero).  Zero for known rows, in the mask column and in rows whose incoming
  * gradients are all zero (whatever their logits hold).  An index outside [0, V)
  * takes no gradient; one that occurs twice takes both.  Columns from V to ldo are not written.
- * dlogits may be the logits themselves. */
+ * dlogits may be the logits themselves (rows at the same places), else no element
+ * of theirs. */
 int mdlm_subs_scores_bwd(const void* logits, int64_t ld, int dtype,
                          const int64_t* xt, const int64_t* x0, const float* lse,
                          const float* entropy, const float* g_logp,

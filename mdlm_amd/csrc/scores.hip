@@ -506,6 +506,7 @@ extern "C" int mdlm_subs_scores_bwd(const void* logits, int64_t ld, int dtype, c
   if (rows == 0) return 0;
   MDLM_CHECK_ARG(logits && xt && x0 && lse && entropy && dlogits, "subs_scores_bwd: null pointer");
   MDLM_CHECK_ARG(rows > 0 && rows < (1ll << 31) && V > 0 && ld >= V && ldo >= V, "subs_scores_bwd: bad shape");
+  MDLM_CHECK_ARG(dlogits != logits || ldo == ld || rows == 1, "subs_scores_bwd: in place, but with rows at other places");
   MDLM_CHECK_ARG(mask_index >= 0 && mask_index < V, "subs_scores_bwd: bad mask index");
   MDLM_CHECK_ARG(top_k >= 0 && top_k <= SC_MAX_K && top_k < V,
                  "subs_scores_bwd: top_k=%d must be at most %d and less than V=%d", top_k, SC_MAX_K, V);

@@ -36,6 +36,7 @@ def _scores_bwd(**kw):
 @pytest.mark.parametrize('bad,text', [
   (dict(logits=0), 'null pointer'), (dict(lse=0), 'null pointer'), (dict(dl=0), 'null pointer'),
   (dict(ti=0), 'alternatives'), (dict(gt=0), 'alternatives'), (dict(ldo=99), 'bad shape'), (dict(ld=99), 'bad shape'),
+  (dict(ldo=101, rows=2), 'in place'),
   (dict(mask=100), 'mask index'), (dict(k=65), 'top_k'), (dict(dtype=7), 'dtype')])
 def test_scores_bwd_refusals(bad, text):
   with pytest.raises(RuntimeError, match=text):
