@@ -526,14 +526,12 @@ int mdlm_adamw_ema(float* p, const float* g, float* m, float* v, float* ema,
  * other indices (-1e6).  A masked row without a finite logit, or with a NaN or
  * +inf outside the mask column, has no distribution: its scores are NaN (lse -inf
  * where every logit is -inf).
- * logits fp32 or bf16, rows `ld` elements apart, aligned to their type.  ws: of
- * mdlm_subs_scores_workspace_bytes (NULL where that is 0); calls that overlap in
- * time need one each. */
+ * logits fp32 or bf16, rows `ld` elements apart, aligned to their type. */
 int mdlm_subs_scores(const void* logits, int64_t ld, int dtype,
                      const int64_t* xt, const int64_t* x0, float* logp,
                      float* entropy, float* lse, float* top_logp,
                      int64_t* top_ids, int64_t rows, int V, int mask_index,
-                     int top_k, void* ws, void* stream);
+                     int top_k, void* stream);
 
 /* Gradient of mdlm_subs_scores with respect to the logits, in their type: lse,
  * entropy, top_ids (rows, top_k) as it left them; g_logp, g_entropy (rows) and
@@ -595,9 +593,7 @@ int mdlm_muon_update(float* p, const float* g, float* m, float* ema,
  *   ln_modulate_bwd, dropout_gate_residual_bwd, colsum_bf16_partial : partial
  *   transpose_bf16      : colsum_partial
  *   masked_row_map      : gather and scatter, each (rows = B*L)
- *   subs_scores         : ws (0: none needed)
  *   orthogonalize       : ws of orthogonalize and muon_update */
-int64_t mdlm_subs_scores_workspace_bytes(int64_t rows, int V, int top_k);
 int64_t mdlm_orthogonalize_workspace_bytes(int n, int rows, int cols);
 int64_t mdlm_attn_bwd_workspace_bytes(int n_seq, int H, int L);
 int64_t mdlm_grad_sumsq_workspace_bytes(void);

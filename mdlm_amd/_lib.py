@@ -65,7 +65,7 @@ SIGNATURES = {
   'mdlm_transpose_bf16': [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp],
   'mdlm_embed_grad': [_vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp],
   'mdlm_subs_nll_bwd': [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp],
-  'mdlm_subs_scores': [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _vp],
+  'mdlm_subs_scores': [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp],
   'mdlm_subs_scores_bwd': [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i32, _i32, _vp],
   'mdlm_orthogonalize': [_vp, _i64, _i64, _i32, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _dbl, _dbl, _dbl, _dbl, _vp, _vp],
   'mdlm_muon_update': [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _i32, _f32, _f32, _f32, _f32, _i32, _dbl, _dbl, _dbl, _dbl,
@@ -83,7 +83,6 @@ SIGNATURES = {
 # workspace-size queries: host arithmetic, return int64 bytes (-1: bad shape)
 SIGNATURES_I64 = {
   'mdlm_attn_bwd_workspace_bytes': [_i32, _i32, _i32],
-  'mdlm_subs_scores_workspace_bytes': [_i64, _i32, _i32],
   'mdlm_orthogonalize_workspace_bytes': [_i32, _i32, _i32],
   'mdlm_grad_sumsq_workspace_bytes': [],
   'mdlm_gemm_bf16_splitk_workspace_bytes': [_i64, _i32, _i32],

@@ -28,7 +28,6 @@ namespace mdlm {
 
 typedef _Float16 f16;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NS_BK = 64;
@@ -46,9 +45,8 @@ static inline NsShape ns_shape(int rows, int cols) {
   q.tall = rows > cols;
   q.s = q.tall ? cols : rows;
   q.l = q.tall ? rows : cols;
-  const int t = 64;      // slabs of the products
-  q.sp = (q.s + t - 1) / t * t;
-  q.lp = (q.l + t - 1) / t * t;
+  q.sp = (q.s + NS_BK - 1) / NS_BK * NS_BK;
+  q.lp = (q.l + NS_BK - 1) / NS_BK * NS_BK;
   return q;
 }
 
@@ -76,8 +74,8 @@ static inline int64_t ns_layout(const NsShape& q, int n, char* base, NsWs* w) {
   return off;
 }
 
-// What is orthogonalised: G itself (MOM = false), or the look-ahead of the momentum
-// of the clipped gradient.
+// What is orthogonalised: G itself, or the look-ahead of the momentum of the clipped
+// gradient.
 struct NsSrc {
   const void* g; int64_t ld, bs; int bf16;
   int rows, cols, vec;      // vec: rows start 16-byte aligned
@@ -348,7 +346,8 @@ __device__ __forceinline__ void slab_wait(int slabs) {
 // N-contiguous operand of APPLY keeps its rows (T columns) and is read through the
 // transposing LDS read (four rows x 16 columns per 16 lanes); its 32-byte blocks
 // are XORed so that the eight rows that half a wave reads fall into different banks.
-// Tiles may reach past M and N: rows and columns are clamped on load, not stored.
+// (APPLY has tiles of 64, 128 and 256.)  Tiles may reach past M and N: rows and columns
+// are clamped on load, not stored.
 template <int MODE, int T, int WM, int WN, int NST>
 struct NsTile {
   static constexpr int OP = T * NS_BK * 2, STAGE = 2 * OP, RING = NST * STAGE;
@@ -359,6 +358,7 @@ struct NsTile {
   static constexpr int PITCH = T + 4, EPI = ER * PITCH; // floats
   static constexpr int LDS = RING > 4 * EPI ? RING : 4 * EPI;
   static __device__ __forceinline__ int block_xor(int row) {
+    static_assert(MODE != NS_APPLY || FN == 2 || FN == 4, "transposing reads below");
     return T % 128 == 0 ? (row & 3) | (((row >> 3) & 1) << 2) : ((row >> 1) & 1) | (((row >> 3) & 1) << 1);
   }
 
@@ -507,10 +507,6 @@ struct NsTile {
                        "s_waitcnt lgkmcnt(0)"
                        : TRO(0), TRO(1), TRO(2), TRO(3)
                        : "v"(tr[0] + o), "v"(tr[1] + o), "v"(tr[2] + o), "v"(tr[3] + o), TRC : "memory");
-        else if constexpr (FN == 3)
-          asm volatile(TR4(0, 1, 2, 3, 12) TR4(4, 5, 6, 7, 13) TR4(8, 9, 10, 11, 14) "s_waitcnt lgkmcnt(0)"
-                       : TRO(0), TRO(1), TRO(2)
-                       : "v"(tr[0] + o), "v"(tr[1] + o), "v"(tr[2] + o), TRC : "memory");
         else
           asm volatile(TR4(0, 1, 2, 3, 8) TR4(4, 5, 6, 7, 9) "s_waitcnt lgkmcnt(0)"
                        : TRO(0), TRO(1)

@@ -711,16 +711,13 @@ def subs_scores(logits, xt, x0, mask_index, top_k=0):
     raise RuntimeError(f'top_k={k}: must be in 0..64 and less than V={V}')
   with _on_device(lg) as stream:
     logp, ent, lse = torch.empty((3, *shape), dtype=torch.float32, device=lg.device).unbind(0)
-    tl = ti = ws = None
+    tl = ti = None
     if k:
       tl = torch.empty((*shape, k), dtype=torch.float32, device=lg.device)
       ti = torch.empty((*shape, k), dtype=torch.int64, device=lg.device)
-    nbytes = _lib.call_i64('mdlm_subs_scores_workspace_bytes', rows, V, k)
-    if nbytes > 0:
-      ws = torch.empty(nbytes, dtype=torch.uint8, device=lg.device)
     call('mdlm_subs_scores', lg.data_ptr(), ld, _DT[lg.dtype], xt.data_ptr(), x0.data_ptr(),
          logp.data_ptr(), ent.data_ptr(), lse.data_ptr(), _p(tl), _p(ti), rows, V,
-         int(mask_index), k, _p(ws), stream)
+         int(mask_index), k, stream)
   return SubsScores(logp, ent, lse, tl, ti)
 
 
