@@ -117,8 +117,13 @@ class Trainer:
       raise ValueError(f'Trainer: optimizer {self.optimizer!r} is neither adamw nor muon')
     self.momentum = float(cfg.optim.get('momentum', 0.95))
     self.ns_steps = int(cfg.optim.get('ns_steps', 5))
+    if not 0 <= self.momentum < 1 or not 1 <= self.ns_steps <= 32:
+      raise ValueError(f'Trainer: optim.momentum={self.momentum} must be in [0, 1), '
+                       f'optim.ns_steps={self.ns_steps} in 1..32')
     self.entropy_weight = float(cfg.training.get('entropy_weight', 0.0)
                                 if entropy_weight is None else entropy_weight)
+    if not math.isfinite(self.entropy_weight):
+      raise ValueError(f'Trainer: entropy_weight={self.entropy_weight} must be finite')
     self.last_entropy = None   # device scalar: mean entropy of the masked positions (entropy_weight != 0)
     self.p_drop = float(bb.blocks[0].dropout if dropout is None else dropout)
     self.ema_decay = float(cfg.training.ema)

@@ -154,6 +154,30 @@ def test_orthogonalize_repeatable_other_stream_and_captured(ops):
     assert torch.equal(out, ops.orthogonalize(g)), i
 
 
+def test_orthogonalize_on_two_streams_at_once(ops):
+  """Calls that overlap in time, each with its own workspace."""
+  g = [gradient(2, 300, 700, seed=90 + i).cuda() for i in range(2)]
+  ref = [ops.orthogonalize(x) for x in g]
+  ws = [torch.empty(ops.workspace_bytes('orthogonalize', 2, 300, 700), dtype=torch.uint8, device='cuda') for _ in g]
+  out = [[torch.empty(2, 300, 700, dtype=torch.bfloat16, device='cuda') for _ in range(6)] for _ in g]
+  side = [torch.cuda.Stream() for _ in g]
+  torch.cuda.synchronize()
+  for k in range(6):
+    for i, s in enumerate(side):
+      with torch.cuda.stream(s):
+        ops.orthogonalize(g[i], out=out[i][k], ws=ws[i])
+  torch.cuda.synchronize()
+  assert all(torch.equal(o, ref[i]) for i in range(2) for o in out[i])
+
+
+def test_orthogonalize_in_place(ops):
+  for shape in ((2, 200, 90), (1, 64, 640)):
+    g = gradient(*shape, seed=4).cuda().bfloat16()
+    ref = ops.orthogonalize(g)
+    assert ops.orthogonalize(g, out=g) is g
+    assert torch.equal(g, ref)
+
+
 def update_oracle(p, g, m, lr, ema, momentum, wd, scale, sumsq, max_norm, grad_scale, omd):
   p, g, m, ema = (t.double() for t in (p, g, m, ema))
   coef = grad_scale

@@ -1,7 +1,6 @@
 """The token scores and the orthogonalised update as a training run uses them
 (Trainer with an entropy term and optimizer 'muon'), and Diffusion.score_tokens."""
 import math
-import os
 
 import pytest
 import torch
@@ -119,6 +118,33 @@ def test_muon_training_steps(ops):
   lg = model.backbone(x0.cuda(), torch.zeros(4, device='cuda')).float().cpu()
   ref = orc.dit_forward({n: v.float() for n, v in P.items()}, x0, torch.zeros(4), cfg.model.n_heads, cfg.model.n_blocks)
   assert _rel(lg, ref) < 2e-2
+
+
+@pytest.mark.parametrize('bad', ['optim.name=sgd', 'optim.momentum=1.0', 'optim.ns_steps=0', 'optim.ns_steps=33',
+                                 'training.entropy_weight=.nan'])
+def test_trainer_refuses(ops, bad):
+  with pytest.raises(ValueError, match=bad.split('=')[0].split('.')[1] if 'name' not in bad else 'sgd'):
+    _make_trainer(0.0, extra=['optim.name=muon', bad])
+
+
+def test_muon_accumulates(ops):
+  """Two micro-batches and one step: the momentum moves by the mean of their gradients."""
+  model, cfg, p, tr = _make_trainer(0.0, extra=['optim.name=muon', 'training.entropy_weight=0.1'])
+  tr.max_norm = 0.0
+  total = None
+  for seed in (1, 2):
+    x0, attn, t, u = (a.cuda() for a in _batch(4, cfg.model.length, seed=seed))
+    tr.forward_backward(x0, attn, t=t, u_xt=u)
+    g = tr.G.double()
+    total = g if total is None else total + g
+  for i, seed in enumerate((1, 2)):
+    x0, attn, t, u = (a.cuda() for a in _batch(4, cfg.model.length, seed=seed))
+    tr.forward_backward(x0, attn, t=t, u_xt=u, accumulate=i > 0, last=i == 1)
+  tr.optimizer_step()
+  for name in ('blocks.0.attn_qkv.weight', 'blocks.1.mlp.2.weight'):
+    o, n, _ = tr.offsets[name]
+    want = total[o:o + n] / 2 * 0.05
+    assert _rel(tr.M1[o:o + n].cpu(), want.cpu()) < 1e-3, name      # atomics order two backward passes
 
 
 def test_muon_checkpoint_resume(ops, tmp_path):
