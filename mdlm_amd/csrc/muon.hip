@@ -408,6 +408,31 @@ struct NsTile {
       for (int n = 0; n < FN; ++n)
         tr[n] = lds0 + OP + row * (2 * T) + (((wc * FN + n) ^ block_xor(row)) * 32) + (lane & 3) * 8;
     }
+    // What an output of the epilogue needs from memory, chunks of 8 of a row: fetched
+    // before the loop where registers allow (64-tiles: few of them run and each waits for
+    // its own latency), else before the sums are turned round.
+    constexpr int CH = T / 8, NC = (ER * CH + THREADS - 1) / THREADS;      // chunks per row, per thread
+    constexpr bool EARLY = T == 64;
+    struct Fetched { f16x8 x[NC]; uint2 lo[NC]; float di[EARLY ? NC : 1]; f32x4 dj[EARLY ? NC : 1][2]; bool ok[NC]; };
+    auto fetch = [&](Fetched& f, int ip) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int q = tid + c * THREADS, i = ip + q / CH, j = j0 + q % CH * 8;
+        f.ok[c] = q < ER * CH && i < g.M && j < g.N;
+        if (MODE != NS_GRAM && f.ok[c]) {
+          const int64_t at = b * g.bso + (int64_t)i * g.ldo + j;
+          f.x[c] = *reinterpret_cast<const f16x8*>((MODE == NS_SQUARE ? g.A : g.B) + at);
+          if (MODE == NS_APPLY) f.lo[c] = *reinterpret_cast<const uint2*>(g.lo + at);
+          if (MODE == NS_SQUARE && EARLY) {
+            f.di[c] = g.diag[b * g.sp + i];
+            f.dj[c][0] = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j);
+            f.dj[c][1] = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j + 4);
+          }
+        }
+      }
+    };
+    Fetched early;
+    if (EARLY) fetch(early, i0);
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int m = 0; m < FM; ++m)
@@ -526,28 +551,16 @@ struct NsTile {
       }
     }
 
-    // ---- epilogue: the sums through LDS, so that global rows are read and written whole.
-    // What an output needs from memory is fetched before the sums are turned round.
+    // ---- epilogue: the sums through LDS, so that global rows are read and written whole
     float* const tile = reinterpret_cast<float*>(smem);
     // the other side of a symmetric product, or a tall matrix's own orientation
     const bool turn = MODE == NS_APPLY ? g.last && g.tall : tm != tn;
-    constexpr int CH = T / 8, NC = (ER * CH + THREADS - 1) / THREADS;      // chunks of 8: per row, per thread
 #pragma unroll
     for (int part = 0; part < T / ER; ++part) {
       const int ip = i0 + part * ER;
-      f16x8 ga[NC];
-      uint2 gb[NC];
-      bool ok[NC];
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int q = tid + c * THREADS, i = ip + q / CH, j = j0 + q % CH * 8;
-        ok[c] = q < ER * CH && i < g.M && j < g.N;
-        if (MODE != NS_GRAM && ok[c]) {
-          const int64_t at = b * g.bso + (int64_t)i * g.ldo + j;
-          ga[c] = *reinterpret_cast<const f16x8*>((MODE == NS_SQUARE ? g.A : g.B) + at);
-          if (MODE == NS_APPLY) gb[c] = *reinterpret_cast<const uint2*>(g.lo + at);
-        }
-      }
+      Fetched late;
+      if (!EARLY) fetch(late, ip);
+      const Fetched& f = EARLY ? early : late;
       __syncthreads();
       if (T == ER || wr * TM / ER == part) {
         float* const own = tile + (wr * TM - part * ER) * PITCH;
@@ -560,7 +573,7 @@ struct NsTile {
       __syncthreads();
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        if (!ok[c]) continue;
+        if (!f.ok[c]) continue;
         const int q = tid + c * THREADS, r = q / CH, pc = q % CH * 8, i = ip + r, j = j0 + pc;
         const int64_t at = b * g.bso + (int64_t)i * g.ldo + j;
         f32x4* const t4 = reinterpret_cast<f32x4*>(tile + r * PITCH + pc);
@@ -581,12 +594,12 @@ struct NsTile {
               }
           }
         } else if constexpr (MODE == NS_SQUARE) {
-          const float di = g.diag[b * g.sp + i];
-          const f32x4 d0 = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j);
-          const f32x4 d1 = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j + 4);
+          const float di = EARLY ? f.di[EARLY ? c : 0] : g.diag[b * g.sp + i];
+          const f32x4 d0 = EARLY ? f.dj[EARLY ? c : 0][0] : *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j);
+          const f32x4 d1 = EARLY ? f.dj[EARLY ? c : 0][1] : *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j + 4);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            x[e] = (x[e] + (di + (e < 4 ? d0[e & 3] : d1[e & 3])) * (float)ga[c][e]) * (g.c / NS_SD);
+            x[e] = (x[e] + (di + (e < 4 ? d0[e & 3] : d1[e & 3])) * (float)f.x[c][e]) * (g.c / NS_SD);
           if (on_diag >= 0 && on_diag < 8) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) if (e == on_diag) x[e] += g.mu * NS_SD;      // (a - b^2/4c) - mu
@@ -594,10 +607,10 @@ struct NsTile {
         } else {
           const float sc = g.last ? 1.f / NS_SX : 1.f;
           float l8[8];
-          unpack_fp8(gb[c], l8);
+          unpack_fp8(f.lo[c], l8);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            x[e] = (g.mu * __builtin_fmaf(l8[e], 1.f / NS_SL, (float)ga[c][e]) + x[e] * (1.f / NS_SD)) * sc;
+            x[e] = (g.mu * __builtin_fmaf(l8[e], 1.f / NS_SL, (float)f.x[c][e]) + x[e] * (1.f / NS_SD)) * sc;
         }
         if (turn) { t4[0] = (f32x4){x[0], x[1], x[2], x[3]}; t4[1] = (f32x4){x[4], x[5], x[6], x[7]}; }
         if (MODE == NS_APPLY && g.last) {
