@@ -28,6 +28,7 @@ namespace mdlm {
 
 typedef _Float16 f16;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NS_BK = 64;
@@ -39,7 +40,9 @@ constexpr float NS_SX = 2048.f;
 constexpr float NS_SD = 256.f;
 constexpr float NS_SL = 16.f;         // of the second word: at most half a step of the first, 8 up to X = 2^14
 
-struct NsShape { int s, l, sp, lp; bool tall; };
+// Short sides up to this many rows (padded): A in parts of K, then one launch for A^2 and P X.
+constexpr int NS_SMALL = 128;
+struct NsShape { int s, l, sp, lp, splits; bool tall; };
 static inline NsShape ns_shape(int rows, int cols) {
   NsShape q;
   q.tall = rows > cols;
@@ -47,6 +50,13 @@ static inline NsShape ns_shape(int rows, int cols) {
   q.l = q.tall ? rows : cols;
   q.sp = (q.s + NS_BK - 1) / NS_BK * NS_BK;
   q.lp = (q.l + NS_BK - 1) / NS_BK * NS_BK;
+  // A part more shortens the chain of slabs (0.2 us each) and is one more to be summed
+  // (us per call, with 4, 5, 8 parts: 128 x 4096: 81, 80, 83; with 11, 16, 16: 128 x 32768:
+  // 174, 179, 179; with 4, 6, 9: 16 x 6000: 72, 67, 67).  By shape alone: a matrix's result
+  // does not depend on how many others it comes with.
+  q.splits = 1;
+  if (q.sp <= NS_SMALL)
+    while (q.splits < 16 && (q.splits + 1) * (q.splits + 1) * (q.sp / 32) <= q.lp / NS_BK) ++q.splits;
   return q;
 }
 
@@ -56,7 +66,8 @@ struct NsWs {
   float* diag;       // n x sp
   f16* h[2];         // n x sp x lp, X's first words
   uint8_t* lo;       // n x sp x lp, its second words
-  f16 *d, *p;        // n x sp x sp
+  f16 *d, *p;        // n x sp x sp, or
+  float* part;       // n x splits x sp x sp
 };
 static inline int64_t ns_layout(const NsShape& q, int n, char* base, NsWs* w) {
   int64_t off = 0;
@@ -68,8 +79,14 @@ static inline int64_t ns_layout(const NsShape& q, int n, char* base, NsWs* w) {
   t.h[0] = (f16*)take(x * 2);
   t.h[1] = (f16*)take(x * 2);
   t.lo = (uint8_t*)take(x);
-  t.d = (f16*)take(d * 2);
-  t.p = (f16*)take(d * 2);
+  t.d = t.p = nullptr;
+  t.part = nullptr;
+  if (q.sp <= NS_SMALL) {
+    t.part = (float*)take(d * q.splits * 4);
+  } else {
+    t.d = (f16*)take(d * 2);
+    t.p = (f16*)take(d * 2);
+  }
   if (w) *w = t;
   return off;
 }
@@ -321,6 +338,7 @@ struct NsGemm {
   f16* out; int64_t ldo, bso;        // D, P or the next X's high words
   uint8_t* lo;                       // APPLY: X's second words, in place
   float* diag; int sp;               // rounding of D's diagonal
+  float* part; int splits;           // GRAM: sums of so many parts of K go here as they are (null: D is made of one)
   float shift, c, mu;                // see the head of this file
   int last, tall;                    // APPLY: the result goes to dst
   NsOut dst;
@@ -362,12 +380,188 @@ struct NsTile {
     return T % 128 == 0 ? (row & 3) | (((row >> 3) & 1) << 2) : ((row >> 1) & 1) | (((row >> 3) & 1) << 1);
   }
 
-  static __device__ __forceinline__ void run(const NsGemm& g, int b, int tm, int tn, char* smem) {
+  static constexpr int CH = T / 8, NC = (ER * CH + THREADS - 1) / THREADS;     // epilogue: chunks per row, per thread
+  // What an output needs from memory (chunks of 8 of a row) is fetched before the loop
+  // where registers allow (64-tiles: few of them run and each waits for its own
+  // latency), else before the sums are turned round.
+  static constexpr bool EARLY = T == 64;
+  struct Fetched { f16x8 x[NC]; uint2 lo[NC]; float di[EARLY ? NC : 1]; f32x4 dj[EARLY ? NC : 1][2]; bool ok[NC]; };
+  static __device__ __forceinline__ void fetch(const NsGemm& g, int b, int i0, int ip, int j0, Fetched& f) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int q = threadIdx.x + c * THREADS, i = ip + q / CH, j = j0 + q % CH * 8;
+      f.ok[c] = q < ER * CH && i < g.M && j < g.N;
+      if (MODE != NS_GRAM && f.ok[c]) {
+        const int64_t at = b * g.bso + (int64_t)i * g.ldo + j;
+        f.x[c] = *reinterpret_cast<const f16x8*>((MODE == NS_SQUARE ? g.A : g.B) + at);
+        if (MODE == NS_APPLY) f.lo[c] = *reinterpret_cast<const uint2*>(g.lo + at);
+        if (MODE == NS_SQUARE && EARLY) {
+          f.di[c] = g.diag[b * g.sp + i];
+          f.dj[c][0] = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j);
+          f.dj[c][1] = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j + 4);
+        }
+      }
+    }
+  }
+
+  // The transposing reads of an N-contiguous slab at `slab`: where this lane's are, and
+  // the fragments of one slab, `o` bytes further.
+  static __device__ __forceinline__ void tr_setup(char* slab, int wc, int lane, unsigned (&tr)[FN]) {
+    const int fr = lane & 15, fq = lane >> 4;
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)slab;
+    const int row = 8 * fq + (fr >> 2);       // + 4, + 32: the same XOR term
+#pragma unroll
+    for (int n = 0; n < FN; ++n)
+      tr[n] = lds0 + row * (2 * T) + (((wc * FN + n) ^ block_xor(row)) * 32) + (lane & 3) * 8;
+  }
+  static __device__ __forceinline__ void read_tr(const unsigned (&tr)[FN], unsigned o, f16x8 (&bf)[2][FN]) {
+    // the reads and their wait in one block: the compiler does not count them
+    uint2 t[2][FN][2];
+#define TR4(d0, d1, d2, d3, a)                                                              \
+  "ds_read_b64_tr_b16 %" #d0 ", %" #a "\n\tds_read_b64_tr_b16 %" #d1 ", %" #a " offset:%c[o4]\n\t" \
+  "ds_read_b64_tr_b16 %" #d2 ", %" #a " offset:%c[o32]\n\tds_read_b64_tr_b16 %" #d3 ", %" #a " offset:%c[o36]\n\t"
+#define TRO(n) "=&v"(t[0][n][0]), "=&v"(t[0][n][1]), "=&v"(t[1][n][0]), "=&v"(t[1][n][1])
+#define TRC [o4] "n"(4 * 2 * T), [o32] "n"(32 * 2 * T), [o36] "n"(36 * 2 * T)
+    if constexpr (FN == 4)
+      asm volatile(TR4(0, 1, 2, 3, 16) TR4(4, 5, 6, 7, 17) TR4(8, 9, 10, 11, 18) TR4(12, 13, 14, 15, 19)
+                   "s_waitcnt lgkmcnt(0)"
+                   : TRO(0), TRO(1), TRO(2), TRO(3)
+                   : "v"(tr[0] + o), "v"(tr[1] + o), "v"(tr[2] + o), "v"(tr[3] + o), TRC : "memory");
+    else
+      asm volatile(TR4(0, 1, 2, 3, 8) TR4(4, 5, 6, 7, 9) "s_waitcnt lgkmcnt(0)"
+                   : TRO(0), TRO(1)
+                   : "v"(tr[0] + o), "v"(tr[1] + o), TRC : "memory");
+#undef TR4
+#undef TRO
+#undef TRC
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int n = 0; n < FN; ++n)
+        bf[ks][n] = __builtin_bit_cast(f16x8, make_uint4(t[ks][n][0].x, t[ks][n][0].y, t[ks][n][1].x, t[ks][n][1].y));
+  }
+
+  // The epilogue: the sums through LDS, so that global rows are read and written whole.
+  static __device__ __forceinline__ void finish(const NsGemm& g, int b, int tm, int tn, int k_part, const Fetched& early,
+                                                const f32x4 (&acc)[FM][FN], char* smem) {
     const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wid / WN, wc = wid % WN, fr = lane & 15, fq = lane >> 4;
     const int i0 = tm * T, j0 = tn * T;
-    const f16* A = g.A + b * g.bsa;
-    const f16* B = g.B + b * g.bsb;
+    float* const tile = reinterpret_cast<float*>(smem);
+    // the other side of a symmetric product, or a tall matrix's own orientation
+    const bool turn = MODE == NS_APPLY ? g.last && g.tall : tm != tn;
+#pragma unroll
+    for (int part = 0; part < T / ER; ++part) {
+      const int ip = i0 + part * ER;
+      Fetched late;
+      if (!EARLY) fetch(g, b, i0, ip, j0, late);
+      const Fetched& f = EARLY ? early : late;
+      __syncthreads();
+      if (T == ER || wr * TM / ER == part) {
+        float* const own = tile + (wr * TM - part * ER) * PITCH;
+#pragma unroll
+        for (int m = 0; m < FM; ++m)
+#pragma unroll
+          for (int n = 0; n < FN; ++n)
+            *reinterpret_cast<f32x4*>(own + (m * 16 + fr) * PITCH + wc * TN + n * 16 + fq * 4) = acc[m][n];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        if (!f.ok[c]) continue;
+        const int q = tid + c * THREADS, r = q / CH, pc = q % CH * 8, i = ip + r, j = j0 + pc;
+        const int64_t at = b * g.bso + (int64_t)i * g.ldo + j;
+        f32x4* const t4 = reinterpret_cast<f32x4*>(tile + r * PITCH + pc);
+        const f32x4 v0 = t4[0], v1 = t4[1];
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = e < 4 ? v0[e & 3] : v1[e & 3];
+        const int on_diag = i - j;                 // 0..7: element of the chunk on the diagonal
+        if (MODE == NS_GRAM && g.part) {
+          float* const to = g.part + (((int64_t)b * g.splits + k_part) * g.sp + i) * g.sp + j;
+          *reinterpret_cast<f32x4*>(to) = v0;
+          *reinterpret_cast<f32x4*>(to + 4) = v1;
+          continue;
+        }
+        if constexpr (MODE == NS_GRAM) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] *= NS_SD / (NS_SX * NS_SX);
+          if (on_diag >= 0 && on_diag < 8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (e == on_diag) {
+                x[e] += g.shift * NS_SD;
+                g.diag[b * g.sp + i] = x[e] - (float)(f16)x[e];
+              }
+          }
+        } else if constexpr (MODE == NS_SQUARE) {
+          const float di = EARLY ? f.di[EARLY ? c : 0] : g.diag[b * g.sp + i];
+          const f32x4 d0 = EARLY ? f.dj[EARLY ? c : 0][0] : *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j);
+          const f32x4 d1 = EARLY ? f.dj[EARLY ? c : 0][1] : *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j + 4);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            x[e] = (x[e] + (di + (e < 4 ? d0[e & 3] : d1[e & 3])) * (float)f.x[c][e]) * (g.c / NS_SD);
+          if (on_diag >= 0 && on_diag < 8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) if (e == on_diag) x[e] += g.mu * NS_SD;      // (a - b^2/4c) - mu
+          }
+        } else {
+          const float sc = g.last ? 1.f / NS_SX : 1.f;
+          float l8[8];
+          unpack_fp8(f.lo[c], l8);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            x[e] = (g.mu * __builtin_fmaf(l8[e], 1.f / NS_SL, (float)f.x[c][e]) + x[e] * (1.f / NS_SD)) * sc;
+        }
+        if (turn) { t4[0] = (f32x4){x[0], x[1], x[2], x[3]}; t4[1] = (f32x4){x[4], x[5], x[6], x[7]}; }
+        if (MODE == NS_APPLY && g.last) {
+          if (!turn) ns_store8(g.dst, b, i, j, x);
+          continue;
+        }
+        f16x8 hv;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) hv[e] = (f16)x[e];
+        *reinterpret_cast<f16x8*>(g.out + at) = hv;
+        if constexpr (MODE == NS_APPLY) {
+          float lv[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) lv[e] = (x[e] - (float)hv[e]) * NS_SL;
+          *reinterpret_cast<uint2*>(g.lo + at) = pack_fp8(lv);
+        }
+      }
+      if (turn && !(MODE == NS_GRAM && g.part)) {      // 16 columns x 4 chunks of 8 rows per wave and pass
+        __syncthreads();
+        constexpr int UNITS = (T / 16) * (ER / 32);
+#pragma unroll 4
+        for (int q = wid; q < UNITS; q += WAVES) {
+          const int jj = (q % (T / 16)) * 16 + fr, ii = (q / (T / 16)) * 32 + fq * 8;
+          const int i = ip + ii, j = j0 + jj;
+          if (i >= g.M || j >= g.N) continue;
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = tile[(ii + e) * PITCH + jj];
+          if constexpr (MODE == NS_APPLY) {
+            ns_store8(g.dst, b, j, i, x);
+          } else {
+            f16x8 hv;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) hv[e] = (f16)x[e];
+            *reinterpret_cast<f16x8*>(g.out + b * g.bso + (int64_t)j * g.ldo + i) = hv;
+          }
+        }
+      }
+    }
+  }
+
+  static __device__ __forceinline__ void run(const NsGemm& g, int b, int tm, int tn, int part, char* smem) {
+    const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wid / WN, wc = wid % WN, fr = lane & 15, fq = lane >> 4;
+    const int i0 = tm * T, j0 = tn * T;
+    // the slabs of this part (GRAM may be split over K)
+    const int KT0 = MODE == NS_GRAM ? part * (g.K / NS_BK) / g.splits : 0;
+    const int KT = (MODE == NS_GRAM ? (part + 1) * (g.K / NS_BK) / g.splits : g.K / NS_BK) - KT0;
+    const f16* A = g.A + b * g.bsa + KT0 * NS_BK;
+    const f16* B = g.B + b * g.bsb + KT0 * NS_BK;
     unsigned aoff[L], boff[L];       // of this lane's 16 bytes of each instruction
 #pragma unroll
     for (int i = 0; i < L; ++i) {
@@ -401,45 +595,15 @@ struct NsTile {
     for (int ks = 0; ks < 2; ++ks) foff[ks] = fr * 128 + (((ks * 4 + fq) ^ (lane & 7)) * 16);
     const int a_base = wr * TM * 128, b_base = OP + wc * TN * 128;
     unsigned tr[FN];
-    if constexpr (MODE == NS_APPLY) {
-      const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)smem;
-      const int row = 8 * fq + (fr >> 2);       // + 4, + 32: the same XOR term
-#pragma unroll
-      for (int n = 0; n < FN; ++n)
-        tr[n] = lds0 + OP + row * (2 * T) + (((wc * FN + n) ^ block_xor(row)) * 32) + (lane & 3) * 8;
-    }
-    // What an output of the epilogue needs from memory, chunks of 8 of a row: fetched
-    // before the loop where registers allow (64-tiles: few of them run and each waits for
-    // its own latency), else before the sums are turned round.
-    constexpr int CH = T / 8, NC = (ER * CH + THREADS - 1) / THREADS;      // chunks per row, per thread
-    constexpr bool EARLY = T == 64;
-    struct Fetched { f16x8 x[NC]; uint2 lo[NC]; float di[EARLY ? NC : 1]; f32x4 dj[EARLY ? NC : 1][2]; bool ok[NC]; };
-    auto fetch = [&](Fetched& f, int ip) {
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int q = tid + c * THREADS, i = ip + q / CH, j = j0 + q % CH * 8;
-        f.ok[c] = q < ER * CH && i < g.M && j < g.N;
-        if (MODE != NS_GRAM && f.ok[c]) {
-          const int64_t at = b * g.bso + (int64_t)i * g.ldo + j;
-          f.x[c] = *reinterpret_cast<const f16x8*>((MODE == NS_SQUARE ? g.A : g.B) + at);
-          if (MODE == NS_APPLY) f.lo[c] = *reinterpret_cast<const uint2*>(g.lo + at);
-          if (MODE == NS_SQUARE && EARLY) {
-            f.di[c] = g.diag[b * g.sp + i];
-            f.dj[c][0] = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j);
-            f.dj[c][1] = *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j + 4);
-          }
-        }
-      }
-    };
+    if constexpr (MODE == NS_APPLY) tr_setup(smem + OP, wc, lane, tr);
     Fetched early;
-    if (EARLY) fetch(early, i0);
+    if (EARLY) fetch(g, b, i0, i0, j0, early);
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int m = 0; m < FM; ++m)
 #pragma unroll
       for (int n = 0; n < FN; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
-    const int KT = g.K / NS_BK;
     auto read_a = [&](const char* sb, int ks, f16x8 (&f)[FM]) {
 #pragma unroll
       for (int m = 0; m < FM; ++m) f[m] = *reinterpret_cast<const f16x8*>(sb + a_base + m * 2048 + foff[ks]);
@@ -519,31 +683,7 @@ struct NsTile {
         f16x8 af[2][FM], bf[2][FN];
         read_a(sb, 0, af[0]);
         read_a(sb, 1, af[1]);
-        // the reads and their wait in one block: the compiler does not count them
-        uint2 t[2][FN][2];
-        const unsigned o = st * STAGE;
-#define TR4(d0, d1, d2, d3, a)                                                              \
-  "ds_read_b64_tr_b16 %" #d0 ", %" #a "\n\tds_read_b64_tr_b16 %" #d1 ", %" #a " offset:%c[o4]\n\t" \
-  "ds_read_b64_tr_b16 %" #d2 ", %" #a " offset:%c[o32]\n\tds_read_b64_tr_b16 %" #d3 ", %" #a " offset:%c[o36]\n\t"
-#define TRO(n) "=&v"(t[0][n][0]), "=&v"(t[0][n][1]), "=&v"(t[1][n][0]), "=&v"(t[1][n][1])
-#define TRC [o4] "n"(4 * 2 * T), [o32] "n"(32 * 2 * T), [o36] "n"(36 * 2 * T)
-        if constexpr (FN == 4)
-          asm volatile(TR4(0, 1, 2, 3, 16) TR4(4, 5, 6, 7, 17) TR4(8, 9, 10, 11, 18) TR4(12, 13, 14, 15, 19)
-                       "s_waitcnt lgkmcnt(0)"
-                       : TRO(0), TRO(1), TRO(2), TRO(3)
-                       : "v"(tr[0] + o), "v"(tr[1] + o), "v"(tr[2] + o), "v"(tr[3] + o), TRC : "memory");
-        else
-          asm volatile(TR4(0, 1, 2, 3, 8) TR4(4, 5, 6, 7, 9) "s_waitcnt lgkmcnt(0)"
-                       : TRO(0), TRO(1)
-                       : "v"(tr[0] + o), "v"(tr[1] + o), TRC : "memory");
-#undef TR4
-#undef TRO
-#undef TRC
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int n = 0; n < FN; ++n)
-            bf[ks][n] = __builtin_bit_cast(f16x8, make_uint4(t[ks][n][0].x, t[ks][n][0].y, t[ks][n][1].x, t[ks][n][1].y));
+        read_tr(tr, st * STAGE, bf);
         mma(af[0], bf[0]);
         mma(af[1], bf[1]);
         st = st + 1 == NST ? 0 : st + 1;
@@ -551,105 +691,7 @@ struct NsTile {
       }
     }
 
-    // ---- epilogue: the sums through LDS, so that global rows are read and written whole
-    float* const tile = reinterpret_cast<float*>(smem);
-    // the other side of a symmetric product, or a tall matrix's own orientation
-    const bool turn = MODE == NS_APPLY ? g.last && g.tall : tm != tn;
-#pragma unroll
-    for (int part = 0; part < T / ER; ++part) {
-      const int ip = i0 + part * ER;
-      Fetched late;
-      if (!EARLY) fetch(late, ip);
-      const Fetched& f = EARLY ? early : late;
-      __syncthreads();
-      if (T == ER || wr * TM / ER == part) {
-        float* const own = tile + (wr * TM - part * ER) * PITCH;
-#pragma unroll
-        for (int m = 0; m < FM; ++m)
-#pragma unroll
-          for (int n = 0; n < FN; ++n)
-            *reinterpret_cast<f32x4*>(own + (m * 16 + fr) * PITCH + wc * TN + n * 16 + fq * 4) = acc[m][n];
-      }
-      __syncthreads();
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        if (!f.ok[c]) continue;
-        const int q = tid + c * THREADS, r = q / CH, pc = q % CH * 8, i = ip + r, j = j0 + pc;
-        const int64_t at = b * g.bso + (int64_t)i * g.ldo + j;
-        f32x4* const t4 = reinterpret_cast<f32x4*>(tile + r * PITCH + pc);
-        const f32x4 v0 = t4[0], v1 = t4[1];
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = e < 4 ? v0[e & 3] : v1[e & 3];
-        const int on_diag = i - j;                 // 0..7: element of the chunk on the diagonal
-        if constexpr (MODE == NS_GRAM) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] *= NS_SD / (NS_SX * NS_SX);
-          if (on_diag >= 0 && on_diag < 8) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (e == on_diag) {
-                x[e] += g.shift * NS_SD;
-                g.diag[b * g.sp + i] = x[e] - (float)(f16)x[e];
-              }
-          }
-        } else if constexpr (MODE == NS_SQUARE) {
-          const float di = EARLY ? f.di[EARLY ? c : 0] : g.diag[b * g.sp + i];
-          const f32x4 d0 = EARLY ? f.dj[EARLY ? c : 0][0] : *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j);
-          const f32x4 d1 = EARLY ? f.dj[EARLY ? c : 0][1] : *reinterpret_cast<const f32x4*>(g.diag + b * g.sp + j + 4);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            x[e] = (x[e] + (di + (e < 4 ? d0[e & 3] : d1[e & 3])) * (float)f.x[c][e]) * (g.c / NS_SD);
-          if (on_diag >= 0 && on_diag < 8) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) if (e == on_diag) x[e] += g.mu * NS_SD;      // (a - b^2/4c) - mu
-          }
-        } else {
-          const float sc = g.last ? 1.f / NS_SX : 1.f;
-          float l8[8];
-          unpack_fp8(f.lo[c], l8);
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            x[e] = (g.mu * __builtin_fmaf(l8[e], 1.f / NS_SL, (float)f.x[c][e]) + x[e] * (1.f / NS_SD)) * sc;
-        }
-        if (turn) { t4[0] = (f32x4){x[0], x[1], x[2], x[3]}; t4[1] = (f32x4){x[4], x[5], x[6], x[7]}; }
-        if (MODE == NS_APPLY && g.last) {
-          if (!turn) ns_store8(g.dst, b, i, j, x);
-          continue;
-        }
-        f16x8 hv;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) hv[e] = (f16)x[e];
-        *reinterpret_cast<f16x8*>(g.out + at) = hv;
-        if constexpr (MODE == NS_APPLY) {
-          float lv[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) lv[e] = (x[e] - (float)hv[e]) * NS_SL;
-          *reinterpret_cast<uint2*>(g.lo + at) = pack_fp8(lv);
-        }
-      }
-      if (turn) {      // 16 columns x 4 chunks of 8 rows per wave and pass
-        __syncthreads();
-        constexpr int UNITS = (T / 16) * (ER / 32);
-#pragma unroll 4
-        for (int q = wid; q < UNITS; q += WAVES) {
-          const int jj = (q % (T / 16)) * 16 + fr, ii = (q / (T / 16)) * 32 + fq * 8;
-          const int i = ip + ii, j = j0 + jj;
-          if (i >= g.M || j >= g.N) continue;
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = tile[(ii + e) * PITCH + jj];
-          if constexpr (MODE == NS_APPLY) {
-            ns_store8(g.dst, b, j, i, x);
-          } else {
-            f16x8 hv;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) hv[e] = (f16)x[e];
-            *reinterpret_cast<f16x8*>(g.out + b * g.bso + (int64_t)j * g.ldo + i) = hv;
-          }
-        }
-      }
-    }
+    finish(g, b, tm, tn, part, early, acc, smem);
   }
 };
 
@@ -666,21 +708,183 @@ template <int MODE, int T, int WM, int WN, int NST>
 __global__ __launch_bounds__(64 * WM * WN, T <= 128 ? 2 : WM * WN / 4) void ns_gemm_kernel(NsGemm g) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tiles_m = (g.M + T - 1) / T, tiles_n = (g.N + T - 1) / T;
-  const int per_mat = MODE == NS_APPLY ? tiles_m * tiles_n : tiles_m * (tiles_m + 1) / 2, total = per_mat * g.n;
+  const int per_mat = MODE == NS_APPLY ? tiles_m * tiles_n : tiles_m * (tiles_m + 1) / 2;
+  const int splits = MODE == NS_GRAM ? g.splits : 1, total = per_mat * splits * g.n;
   // each XCD (workgroup id & 7) gets a contiguous range of tiles
   const int per_xcd = (total + 7) >> 3;
   const int idx = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
   if ((int)(blockIdx.x >> 3) >= per_xcd || idx >= total) return;
-  const int b = idx / per_mat, t = idx - b * per_mat;
+  const int u = idx / per_mat, t = idx - u * per_mat, b = u / splits, part = u - b * splits;
   int tm, tn;
   if (MODE == NS_APPLY) { tn = t / tiles_m; tm = t - tn * tiles_m; }     // X's columns are read once per XCD
   else triangle(t, tm, tn);
-  NsTile<MODE, T, WM, WN, NST>::run(g, b, tm, tn, smem);
+  NsTile<MODE, T, WM, WN, NST>::run(g, b, tm, tn, part, smem);
+}
+
+// SQUARE and APPLY of matrices whose short side fits into 128 rows, in one launch: a
+// launch costs 4 us there, the products next to nothing (us per call, three launches per
+// step / two: 2 x 384 x 128: 67 / 60, 128 x 4096: 124 / 81, 16 x 6000: 141 / 67,
+// 300 x 100 x 140: 202 / 174, 64 x 128 x 2048: 200 / 204).  Every workgroup sums D from the
+// parts that GRAM left, makes 64 rows of P in LDS and multiplies `group` 64 x 64 tiles of X
+// by them, the next one's X on its way meanwhile.  LDS rows as in NsTile.
+template <int S>
+__global__ __launch_bounds__(256) void ns_step_kernel(NsGemm g, float p_diag, int group) {
+  using Tile = NsTile<NS_APPLY, 64, 2, 2, 4>;
+  constexpr int KS = S / 64, DSLAB = S * 128, SLAB = 64 * 128;
+  // D; later the epilogue's tile and X's second buffer
+  constexpr int DBYTES = KS * DSLAB > 4 * Tile::EPI + KS * SLAB ? KS * DSLAB : 4 * Tile::EPI + KS * SLAB;
+  __shared__ __attribute__((aligned(16))) char dm[DBYTES];
+  __shared__ __attribute__((aligned(16))) char xs[KS * SLAB];
+  __shared__ __attribute__((aligned(16))) char ps[KS * SLAB];
+  __shared__ __attribute__((aligned(16))) float diag[S];
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wid >> 1, wc = wid & 1, fr = lane & 15, fq = lane >> 4;
+  const int tiles_n = g.N / 64, per_mat = KS * ((tiles_n + group - 1) / group), total = per_mat * g.n, per_xcd = (total + 7) >> 3;
+  const int idx = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per_xcd || idx >= total) return;
+  const int b = idx / per_mat, t = idx - b * per_mat, grp = t / KS, tm = t - grp * KS;
+  const int i0 = tm * 64, tn0 = grp * group, tn1 = tn0 + group < tiles_n ? tn0 + group : tiles_n;
+  const f16* X = g.B + b * g.bsb;
+  auto stage = [&](int tn, char* to) {
+#pragma unroll
+    for (int kt = 0; kt < KS; ++kt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int q = (i * 4 + wid) * 64 + lane, k = q >> 3, pch = q & 7;
+        const int j = (((pch >> 1) ^ Tile::block_xor(k)) * 2 + (pch & 1)) * 8;
+        NS_GLDS16(X + (int64_t)(kt * 64 + k) * g.ldb + tn * 64 + j, to + kt * SLAB + (i * 4 + wid) * 1024);
+      }
+  };
+  typename Tile::Fetched own;
+  Tile::fetch(g, b, i0, i0, tn0 * 64, own);
+  stage(tn0, xs);
+  // ---- D: the lower triangle's tiles (0,0), (1,0), (1,1), two chunks of 8 per thread and tile
+  constexpr int C = KS * (KS + 1);
+  f32x4 v[C][2];
+#pragma unroll
+  for (int c = 0; c < C; ++c) v[c][0] = v[c][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < g.splits; ++p) {
+    const float* part = g.part + ((int64_t)b * g.splits + p) * (S * S);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int q = tid + (c & 1) * 256, i = (c > 1 ? 64 : 0) + (q >> 3), j = (c > 3 ? 64 : 0) + (q & 7) * 8;
+      v[c][0] += *reinterpret_cast<const f32x4*>(part + i * S + j);
+      v[c][1] += *reinterpret_cast<const f32x4*>(part + i * S + j + 4);
+    }
+  }
+  auto at = [](int row, int col, int slab) { return (col >> 6) * slab + row * 128 + ((((col >> 3) & 7) ^ (row & 7)) * 16) + (col & 7) * 2; };
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const int q = tid + (c & 1) * 256, i = (c > 1 ? 64 : 0) + (q >> 3), j = (c > 3 ? 64 : 0) + (q & 7) * 8;
+    f16x8 h;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float x = v[c][e >> 2][e & 3] * (NS_SD / (NS_SX * NS_SX));
+      if (i == j + e) x += g.shift * NS_SD;
+      h[e] = (f16)x;
+      if (i == j + e) diag[i] = x - (float)h[e];
+    }
+    *reinterpret_cast<f16x8*>(dm + at(i, j, DSLAB)) = h;
+    if (c == 2 || c == 3) {       // the other side
+#pragma unroll
+      for (int e = 0; e < 8; ++e) *reinterpret_cast<f16*>(dm + at(j + e, i, DSLAB)) = h[e];
+    }
+  }
+  slab_wait<0, 0>(0);
+  // ---- P, 64 rows of it
+  constexpr int FN = S / 32;
+  {
+    f32x4 acc[2][FN];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < FN; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < 2 * KS; ++ks) {
+      f16x8 fa[2], fb[FN];
+      const int col = ks * 32 + fq * 8;
+#pragma unroll
+      for (int m = 0; m < 2; ++m) fa[m] = *reinterpret_cast<const f16x8*>(dm + at(i0 + wr * 32 + m * 16 + fr, col, DSLAB));
+#pragma unroll
+      for (int n = 0; n < FN; ++n) fb[n] = *reinterpret_cast<const f16x8*>(dm + at(wc * (S / 2) + n * 16 + fr, col, DSLAB));
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int n = 0; n < FN; ++n)
+          acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[n], fa[m], acc[m][n], 0, 0, 0);
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < FN; ++n) {
+        const int r = wr * 32 + m * 16 + fr, i = i0 + r, j = wc * (S / 2) + n * 16 + fq * 4;
+        const f16x4 d = *reinterpret_cast<const f16x4*>(dm + at(i, j, DSLAB));
+        const float di = diag[i];
+        const f32x4 dj = *reinterpret_cast<const f32x4*>(diag + j);
+        f16x4 h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = (acc[m][n][e] + (di + dj[e]) * (float)d[e]) * (g.c / NS_SD);
+          if (i == j + e) x += p_diag * NS_SD;
+          h[e] = (f16)x;
+        }
+        *reinterpret_cast<f16x4*>(ps + at(r, j, SLAB)) = h;
+      }
+  }
+  // ---- P X
+  for (int tn = tn0; tn < tn1; ++tn) {
+    // this tile's X has landed and the other buffer is free (first time: P is there, D done with)
+    slab_wait<0, 0>(0);
+    char* const cur = (tn - tn0) & 1 ? dm + 4 * Tile::EPI : xs;
+    typename Tile::Fetched next;
+    if (tn + 1 < tn1) {
+      Tile::fetch(g, b, i0, i0, (tn + 1) * 64, next);
+      stage(tn + 1, (tn - tn0) & 1 ? xs : dm + 4 * Tile::EPI);
+    }
+    f32x4 acc[2][2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) acc[m][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    unsigned tr[2];
+    Tile::tr_setup(cur, wc, lane, tr);
+#pragma unroll
+    for (int kt = 0; kt < KS; ++kt) {
+      f16x8 bf[2][2];
+      Tile::read_tr(tr, kt * SLAB, bf);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const f16x8 fa = *reinterpret_cast<const f16x8*>(ps + at(wr * 32 + m * 16 + fr, kt * 64 + ks * 32 + fq * 8, SLAB));
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+            acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf[ks][n], fa, acc[m][n], 0, 0, 0);
+        }
+    }
+    Tile::finish(g, b, tm, tn, 0, own, acc, dm);
+    own = next;
+  }
+}
+static int ns_step(const NsGemm& g, float p_diag, int cus, hipStream_t st) {
+  // as many tiles per workgroup as leave two workgroups per CU (what LDS has room for); us per
+  // call with one tile each / four workgroups per CU / two / one: 64 x 128 x 2048:
+  // 405 / 228 / 204 / 234, 4 x 128 x 8192: 177 / 167 / 131 / 131
+  const int tiles_n = g.N / 64;
+  int64_t group = ((int64_t)(g.M / 64) * tiles_n * g.n + 2 * cus - 1) / (2 * cus);
+  if (group > tiles_n) group = tiles_n;
+  const int64_t total = (int64_t)(g.M / 64) * ((tiles_n + group - 1) / group) * g.n;
+  if (total >= (1ll << 28)) { set_error("orthogonalize: too many tiles"); return -1; }
+  const unsigned grid = (unsigned)((total + 7) / 8 * 8);
+  if (g.M == 64) ns_step_kernel<64><<<grid, 256, 0, st>>>(g, p_diag, (int)group);
+  else ns_step_kernel<128><<<grid, 256, 0, st>>>(g, p_diag, (int)group);
+  MDLM_LAUNCH_CHECK();
+  return 0;
 }
 
 static int64_t ns_tiles(int mode, const NsGemm& g, int T) {
   const int64_t tm = (g.M + T - 1) / T, tn = (g.N + T - 1) / T;
-  return (mode == NS_APPLY ? tm * tn : tm * (tm + 1) / 2) * g.n;
+  return (mode == NS_APPLY ? tm * tn : tm * (tm + 1) / 2 * (mode == NS_GRAM ? g.splits : 1)) * g.n;
 }
 template <int MODE, int T, int WM, int WN, int NST>
 static int ns_launch(const NsGemm& g, hipStream_t st) {
@@ -755,18 +959,20 @@ static int ns_run(NsSrc src, NsOut dst, int n, int rows, int cols, int steps, do
     const double mu = it + 2 < steps ? a : 1.0;
     f16 *x = w.h[it & 1], *xn = w.h[(it & 1) ^ 1];
     NsGemm g = {};
-    g.n = n; g.sp = q.sp; g.diag = w.diag;
+    g.n = n; g.sp = q.sp; g.diag = w.diag; g.part = w.part; g.splits = q.splits;
     g.A = x; g.lda = q.lp; g.bsa = bx; g.B = x; g.ldb = q.lp; g.bsb = bx; g.K = q.lp;
     g.M = g.N = q.sp;
     g.out = w.d; g.ldo = q.sp; g.bso = bd; g.shift = (float)(b / (2 * c));
-    if (int rc = ns_gemm<NS_GRAM>(g, cus, st)) return rc;
+    const float p_diag = (float)(a - b * b / (4 * c) - mu);
+    if (int rc = w.part ? ns_launch<NS_GRAM, 64, 2, 2, 4>(g, st) : ns_gemm<NS_GRAM>(g, cus, st)) return rc;
     g.A = w.d; g.lda = q.sp; g.bsa = bd; g.B = w.d; g.ldb = q.sp; g.bsb = bd; g.K = q.sp;
-    g.out = w.p; g.c = (float)c; g.mu = (float)(a - b * b / (4 * c) - mu);
-    if (int rc = ns_gemm<NS_SQUARE>(g, cus, st)) return rc;
+    g.out = w.p; g.c = (float)c; g.mu = p_diag;
+    if (!w.part)
+      if (int rc = ns_gemm<NS_SQUARE>(g, cus, st)) return rc;
     g.A = w.p; g.B = x; g.ldb = q.lp; g.bsb = bx; g.N = q.lp;
     g.out = xn; g.ldo = q.lp; g.bso = bx; g.lo = w.lo; g.mu = (float)mu;
     g.last = it + 1 == steps; g.tall = q.tall; g.dst = dst;
-    if (int rc = ns_gemm<NS_APPLY>(g, cus, st)) return rc;
+    if (int rc = w.part ? ns_step(g, p_diag, cus, st) : ns_gemm<NS_APPLY>(g, cus, st)) return rc;
   }
   return 0;
 }

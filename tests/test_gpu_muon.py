@@ -53,7 +53,8 @@ def gradient(n, r, c, seed, decay=0.0):
 
 
 SHAPES = [(1, 1, 1), (1, 1, 7), (1, 5, 1), (2, 3, 3), (1, 16, 200), (1, 127, 129), (1, 128, 128), (2, 129, 64),
-          (3, 200, 333), (1, 517, 130), (2, 384, 128), (1, 1000, 300), (1, 640, 1291), (3, 128, 512), (2, 512, 100), (2, 129, 512),
+          (3, 200, 333), (1, 517, 130), (2, 384, 128), (1, 1000, 300), (1, 640, 1291), (3, 128, 512), (2, 512, 100),
+          (2, 129, 512),
           (1, 100, 513), (5, 33, 250), (2, 257, 17), (1, 129, 129)]
 
 
@@ -67,6 +68,19 @@ def test_orthogonalize(ops, n, r, c, dtype):
     want = oracle(g)
     for i in range(n):
       assert rel(got[i], want[i]) < tol_factor(5) + 2.0 ** -8, (i, decay)
+
+
+@pytest.mark.parametrize('n,r,c', [(1, 1, 6000), (1, 64, 513), (1, 30, 4100), (1, 128, 5000), (2, 100, 1025),
+                                   (1, 9000, 65), (3, 2100, 128), (40, 70, 2000), (5, 16, 20000), (9, 128, 8200),
+                                   (600, 128, 66)])
+def test_orthogonalize_short_sides(ops, n, r, c):
+  """Short sides of up to 128 rows: A summed in parts of the long side, and workgroups
+  that go through several tiles of X, the last ones fewer."""
+  g = gradient(n, r, c, seed=r)
+  got = ops.orthogonalize(g.cuda())
+  for i in {0, n // 2, n - 1}:
+    assert rel(got[i], oracle(g[i])) < tol_factor(5) + 2.0 ** -8, i
+    assert torch.equal(got[i], ops.orthogonalize(g[i].cuda())), i
 
 
 @pytest.mark.parametrize('n,r,c', [(300, 100, 140), (40, 560, 600), (25, 1000, 990), (30, 1100, 300), (20, 450, 500)])
