@@ -279,3 +279,24 @@ def test_muon_update_captured(ops):
     torch.cuda.synchronize()
     step(q, k)
     assert torch.equal(p, q) and torch.equal(m, k), i
+
+
+def test_past_32_bit_offsets(ops):
+  """Matrices, and rows of one, more than 2^31 elements apart: moved as they are side by side."""
+  n, r, c, far = 2, 70, 140, 2 ** 31 + 64
+  flat = {k: torch.empty(far + 70 * 200, dtype=torch.bfloat16 if k == 'w' else torch.float32, device='cuda')
+          for k in 'pgmew'}
+  gen = torch.Generator().manual_seed(3)
+  near = {k: (torch.randn(n, r, c, generator=gen) * 0.1).cuda() for k in 'pgme'}
+  near['w'] = near['p'].to(torch.bfloat16)
+  away = {k: t.as_strided((n, r, c), (far, 200, 1)) for k, t in flat.items()}
+  for k in away:
+    away[k].copy_(near[k])
+  assert torch.equal(ops.orthogonalize(away['g']), ops.orthogonalize(near['g']))
+  for v in (away, near):
+    ops.muon_update(v['p'], v['g'], v['m'], 1e-2, ema=v['e'], w16=v['w'], ema_one_minus_decay=0.1)
+  assert all(torch.equal(away[k], near[k]) for k in near)
+  rows = flat['p'].as_strided((2, 50), (far, 1))
+  assert torch.equal(ops.orthogonalize(rows), ops.orthogonalize(rows.contiguous()))
+  wide = ops.orthogonalize(away['g'], out=away['w'])
+  assert wide is away['w'] and torch.equal(wide, ops.orthogonalize(near['g']))
