@@ -208,6 +208,14 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsSrc a, double* __restric
   if (threadIdx.x == 0) part[(int64_t)b * NS_MAX_PARTS + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
+// A value that is split into words, or written twice, as one fp32 number.  Left to itself
+// the compiler folds the operation that made it into one of its conversions to fp16 and not
+// into the other: where that moves a tie (one element in 2^13) the rest is taken against another
+// first word than the stored one, and a whole step of fp16 is lost.
+__device__ __forceinline__ float pinned(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
 __device__ __forceinline__ uint2 pack_fp8(const float (&v)[8]) {
   int a = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
   a = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], a, true);
@@ -266,7 +274,7 @@ __global__ __launch_bounds__(256) void ns_ingest_kernel(NsSrc a, const double* _
     float lv[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float f = (tall ? tile[y][x + e] : v[k][e]) * inv;
+      const float f = pinned((tall ? tile[y][x + e] : v[k][e]) * inv);
       hv[e] = (f16)f;
       lv[e] = (f - (float)hv[e]) * NS_SL;
     }
@@ -490,7 +498,7 @@ struct NsTile {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
               if (e == on_diag) {
-                x[e] += g.shift * NS_SD;
+                x[e] = pinned(x[e] + g.shift * NS_SD);
                 g.diag[b * g.sp + i] = x[e] - (float)(f16)x[e];
               }
           }
@@ -513,6 +521,8 @@ struct NsTile {
           for (int e = 0; e < 8; ++e)
             x[e] = (g.mu * __builtin_fmaf(l8[e], 1.f / NS_SL, (float)f.x[c][e]) + x[e] * (1.f / NS_SD)) * sc;
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = pinned(x[e]);
         if (turn) { t4[0] = (f32x4){x[0], x[1], x[2], x[3]}; t4[1] = (f32x4){x[4], x[5], x[6], x[7]}; }
         if (MODE == NS_APPLY && g.last) {
           if (!turn) ns_store8(g.dst, b, i, j, x);
@@ -781,6 +791,7 @@ __global__ __launch_bounds__(256) void ns_step_kernel(NsGemm g, float p_diag, in
     for (int e = 0; e < 8; ++e) {
       float x = v[c][e >> 2][e & 3] * (NS_SD / (NS_SX * NS_SX));
       if (i == j + e) x += g.shift * NS_SD;
+      x = pinned(x);
       h[e] = (f16)x;
       if (i == j + e) diag[i] = x - (float)h[e];
     }
