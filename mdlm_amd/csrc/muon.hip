@@ -11,9 +11,9 @@
 //   P = c D D^T + (a - b^2/4c) I,   X <- mu X + (P - mu I) X.
 // mu = a in the early steps (small singular values: P is close to a I) and 1 in
 // the last two (P is close to I), and the mu X term takes X from two words, fp16 and
-// e4m3 (15 bits together: 16 more bits of the second word change nothing, and it is a
-// third of what the products move), so that only the small P - mu I sees X rounded
-// to fp16.  Without the second word matrices of fast decaying spectra lose: 3e-3.
+// e4m3 (15 bits together: 8 more bits of the second word take a decaying spectrum from 1.0e-3
+// to 9.6e-4, and it is a third of what the products move), so that only the small P - mu I
+// sees X rounded to fp16.  Without the second word matrices of fast decaying spectra lose: 1.2e-2.
 // The diagonal of D, its largest part, is also corrected for its rounding:
 // d = D_ii - fp16(D_ii) enters D D^T to first order.  Against 64 bits the result is
 // 4e-4 .. 1e-3 off (2-norm, relative), less than rounding it to bf16 costs
@@ -38,7 +38,12 @@ constexpr int NS_MAX_PARTS = 1024;    // partial sums of |G|^2 per matrix, at mo
 // most a few units.
 constexpr float NS_SX = 2048.f;
 constexpr float NS_SD = 256.f;
-constexpr float NS_SL = 16.f;         // of the second word: at most half a step of the first, 8 up to X = 2^14
+// Of the second word, what X loses in the first: at most 1 while the first is below 2^12, |X| < 2.
+// e4m3 goes from 2^-9 to 448, so 256 keeps the most of it that large matrices need, whose entries
+// are small (average of X_0 at 4096 x 8192: 0.35 with NS_SX).  Off by (decaying spectra, i^-1.5, of 1024 x 4096,
+// 4096 x 8192, 16384 x 32768) with 16: 2.0e-3, 4.6e-3, 1.0e-2, with 256: 1.0e-3, 1.0e-3, 1.7e-3.
+constexpr float NS_SL = 256.f;
+constexpr float NS_LO_MAX = 448.f;    // larger X lose bits of the second word, no more
 
 // Short sides up to this many rows (padded): A in parts of K, then one launch for A^2 and P X.
 constexpr int NS_SMALL = 128;
@@ -216,7 +221,10 @@ __device__ __forceinline__ float pinned(float x) {
   asm("" : "+v"(x));
   return x;
 }
-__device__ __forceinline__ uint2 pack_fp8(const float (&v)[8]) {
+__device__ __forceinline__ uint2 pack_fp8(const float (&x)[8]) {
+  float v[8];       // past the largest e4m3 the conversion gives NaN
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = __builtin_amdgcn_fmed3f(x[e], -NS_LO_MAX, NS_LO_MAX);
   int a = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false);
   a = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], a, true);
   int b = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);

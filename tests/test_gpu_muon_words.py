@@ -48,3 +48,30 @@ def test_two_words(ops, n, r, c, steps):
   want = A ** steps * x0(g)
   err, tol = (got - want).abs(), steps * (REL * want.abs() + 2.0 ** -25)
   assert (err <= tol).all(), f'{int((err > tol).sum())} elements, up to {(err / tol).max().item():.3g} times the bound'
+
+
+@pytest.mark.parametrize('n,r,c', [(1, 4096, 8192), (1, 1500, 20000), (1, 6000, 3001)])
+def test_two_words_of_large_matrices(ops, n, r, c):
+  """Their entries are small, and the second word is still there: half its smallest
+  step is 2^-10 / (256 x 2048) = 2^-29."""
+  gen = torch.Generator(device='cuda').manual_seed(r + c)
+  g = torch.randn(n, r, c, generator=gen, device='cuda')
+  got = move(ops, g, steps=2, coeffs=(A, 0.0, 1e-6)).double()
+  want = A ** 2 * x0(g)
+  err, tol = (got - want).abs(), 2 * (REL * want.abs() + 2.0 ** -29)
+  assert (err <= tol).all(), f'{int((err > tol).sum())} elements, up to {(err / tol).max().item():.3g} times the bound'
+
+
+def test_two_words_of_large_entries(ops):
+  """A single entry is X_0 = 1, the largest there is.  With a = 2.4 it is 5.76 before the third
+  step, where what the first word leaves, 3.5 of 11796, times 256 is past the largest e4m3:
+  cut off there, no NaN, and no more lost than the first words' half steps (and those
+  of P), 2^-11 each; c A^2 adds 1e-7 x 5.76^4."""
+  g = torch.zeros(2, 70, 90, device='cuda')
+  g[0, 3, 5] = 0.7
+  g[1, 69, 89] = -4e-3
+  o = move(ops, g, steps=3, coeffs=(2.4, 0.0, 1e-7))
+  for got, want in ((o[0, 3, 5], 2.4 ** 3), (o[1, 69, 89], -2.4 ** 3)):
+    assert abs(got.item() / want - 1) <= 3 * 2 * 2.0 ** -11 + 1.2e-4
+  o[0, 3, 5] = o[1, 69, 89] = 0
+  assert (o == 0).all()
