@@ -9,15 +9,19 @@
 //   a + b t + c t^2 = c (t + b/2c)^2 + (a - b^2/4c),
 // D = A + (b/2c) I is small near convergence and nothing cancels:
 //   P = c D D^T + (a - b^2/4c) I,   X <- mu X + (P - mu I) X.
-// mu = a in the early steps (small singular values: P is close to a I) and 1 in
-// the last two (P is close to I), and the mu X term takes X from two words, fp16 and
+// mu = a in the early steps (small singular values: P is close to a I), 1 in the last one
+// (P is close to I) and half way in the one before, when some values have arrived and some are
+// still small (1 there: 1.9e-3 instead of 1.1e-3 off for low rank and noise, 4096 x 8192, and
+// 20 % more on average over shapes and spectra).  The mu X term takes X from two words, fp16 and
 // e4m3 (15 bits together: 8 more bits of the second word take a decaying spectrum from 1.0e-3
 // to 9.6e-4, and it is a third of what the products move), so that only the small P - mu I
 // sees X rounded to fp16.  Without the second word matrices of fast decaying spectra lose: 1.2e-2.
 // The diagonal of D, its largest part, is also corrected for its rounding:
-// d = D_ii - fp16(D_ii) enters D D^T to first order.  Against 64 bits the result is
-// 4e-4 .. 1e-3 off (2-norm, relative), less than rounding it to bf16 costs
-// (1.7e-3); plain bf16 operands are 1e-2 .. 3e-2 off.
+// d = D_ii - fp16(D_ii) enters D D^T to first order.  Against 64 bits the result of five steps is
+// 3e-4 .. 1.3e-3 off (2-norm, relative; sides of up to 64 rows up to 1.6e-3, 16384 x 32768 with a
+// spectrum of i^-1.5 1.5e-3), less than rounding it to bf16 costs (1.7e-3); plain bf16 operands
+// are 1e-2 .. 3e-2 off.  The usual coefficients do not converge: a step more makes differences
+// larger (6 steps up to 2e-3, 7 3e-3, 10 1.5e-2), as it does to those of the input.
 //
 // Every matrix is padded with zeros to whole slabs of 64 in the workspace; padding
 // stays zero through every step.
@@ -975,7 +979,7 @@ static int ns_run(NsSrc src, NsOut dst, int n, int rows, int cols, int steps, do
   MDLM_LAUNCH_CHECK();
   const int64_t bx = (int64_t)q.sp * q.lp, bd = (int64_t)q.sp * q.sp;
   for (int it = 0; it < steps; ++it) {
-    const double mu = it + 2 < steps ? a : 1.0;
+    const double mu = it + 2 < steps ? a : it + 2 == steps ? 0.5 * (a + 1.0) : 1.0;
     f16 *x = w.h[it & 1], *xn = w.h[(it & 1) ^ 1];
     NsGemm g = {};
     g.n = n; g.sp = q.sp; g.diag = w.diag; g.part = w.part; g.splits = q.splits;

@@ -62,3 +62,16 @@ def check(ops, g):
 @pytest.mark.parametrize('r,c', [(256, 512), (128, 1024), (640, 1291), (4096, 1024), (2048, 8192), (4096, 8192)])
 def test_decaying_spectrum(ops, r, c):
   check(ops, decaying(r, c))
+
+
+def low_rank(r, c, seed=0):
+  """A signal of rank min/16 and noise of 2 % of its size."""
+  gen = torch.Generator(device='cuda').manual_seed(seed)
+  k = min(r, c) // 16
+  signal = torch.randn(r, k, generator=gen, device='cuda') @ torch.randn(k, c, generator=gen, device='cuda')
+  return signal / math.sqrt(k) + 0.02 * torch.randn(r, c, generator=gen, device='cuda')
+
+
+@pytest.mark.parametrize('r,c', [(256, 512), (128, 1024), (1024, 4096), (8192, 2048), (4096, 8192)])
+def test_low_rank_and_noise(ops, r, c):
+  check(ops, low_rank(r, c))
