@@ -555,7 +555,9 @@ int mdlm_subs_scores_bwd(const void* logits, int64_t ld, int dtype,
  * is AdamW, diffusion.py:449-459).  n matrices (rows, cols), fp32 or bf16, rows
  * `ld` and matrices `stride` elements apart; out bf16 (the products round their
  * operands to fp16: the result is good to bf16).  |a| <= 16, 0 < |c| <= 32, |b^2 / 4c| <= 16,
- * steps <= 32; |G|_F + eps counts as at least 6.1e-36.
+ * steps <= 32, and coefficients that take a singular value from [0, 1] past 31 before the last
+ * step, or its square t, |t + b / 2c| or |a + b t + c t^2 - 1| past 248, are refused (fp16
+ * holds no more); |G|_F + eps counts as at least 6.1e-36.
  * `out` may be g itself.  ws: mdlm_orthogonalize_workspace_bytes(n, rows, cols),
  * 256-byte aligned; calls that overlap in time (two streams, two captured graphs
  * replayed at once) need one each. */

@@ -956,6 +956,31 @@ static int ns_gemm(const NsGemm& g, int cus, hipStream_t st) {
   return c256 < c128 ? ns_launch<MODE, 256, 2, 4, 2>(g, st) : ns_launch<MODE, 128, 2, 2, 2>(g, st);
 }
 
+static inline double ns_mu(int it, int steps, double a) {
+  return it + 2 < steps ? a : it + 2 == steps ? 0.5 * (a + 1.0) : 1.0;
+}
+// Whether X, D and P - mu I stay in the range of fp16 with their scales, whatever the matrix:
+// an entry is at most the largest singular value, X_0's are in [0, 1], and each step maps [0, s]
+// by s p(s^2), p(t) = a + b t + c t^2, which has its extremes at the ends and where its derivative is 0.
+static bool ns_in_range(int steps, double a, double b, double c) {
+  const double most_x = 65504 / NS_SX * 0.97, most_p = 65504 / NS_SD * 0.97;      // less what roundings add
+  double s = 1.0;
+  for (int it = 0; it < steps; ++it) {
+    const double t = s * s, mu = ns_mu(it, steps, a), shift = b / (2 * c);
+    auto p = [&](double u) { return a + u * (b + c * u); };
+    double dp = fmax(fabs(a - mu), fabs(p(t) - mu));
+    if (-shift > 0 && -shift < t) dp = fmax(dp, fabs(p(-shift) - mu));
+    if (!(fmax(fabs(shift), fmax(fabs(t + shift), t)) < most_p) || !(dp < most_p)) return false;
+    double next = fabs(s * p(t));
+    const double disc = 9 * b * b - 20 * a * c;
+    if (disc >= 0)
+      for (double u : {(-3 * b + sqrt(disc)) / (10 * c), (-3 * b - sqrt(disc)) / (10 * c)})
+        if (u > 0 && u < t) next = fmax(next, fabs(sqrt(u) * p(u)));
+    s = next;
+    if (it + 1 < steps && !(s < most_x)) return false;
+  }
+  return true;
+}
 static int ns_run(NsSrc src, NsOut dst, int n, int rows, int cols, int steps, double a, double b, double c,
                   double eps, void* ws, hipStream_t st) {
   const int dev = current_device();
@@ -979,7 +1004,7 @@ static int ns_run(NsSrc src, NsOut dst, int n, int rows, int cols, int steps, do
   MDLM_LAUNCH_CHECK();
   const int64_t bx = (int64_t)q.sp * q.lp, bd = (int64_t)q.sp * q.sp;
   for (int it = 0; it < steps; ++it) {
-    const double mu = it + 2 < steps ? a : it + 2 == steps ? 0.5 * (a + 1.0) : 1.0;
+    const double mu = ns_mu(it, steps, a);
     f16 *x = w.h[it & 1], *xn = w.h[(it & 1) ^ 1];
     NsGemm g = {};
     g.n = n; g.sp = q.sp; g.diag = w.diag; g.part = w.part; g.splits = q.splits;
@@ -1012,6 +1037,8 @@ static int ns_check(const char* who, int n, int rows, int cols, int64_t ld, int6
   MDLM_CHECK_ARG(isfinite(a) && isfinite(b) && isfinite(c) && fabs(a) <= 16 && c != 0.0 && fabs(c) <= 32 &&
                    fabs(b * b / (4 * c)) <= 16,
                  "%s: coefficients (%g, %g, %g) are outside what the fp16 products hold", who, a, b, c);
+  MDLM_CHECK_ARG(ns_in_range(steps, a, b, c),
+                 "%s: coefficients (%g, %g, %g) can leave the range of the fp16 products in %d steps", who, a, b, c, steps);
   MDLM_CHECK_ARG(eps > 0.0 && isfinite(eps), "%s: eps must be positive", who);
   return 0;
 }

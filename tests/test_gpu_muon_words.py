@@ -75,3 +75,30 @@ def test_two_words_of_large_entries(ops):
     assert abs(got.item() / want - 1) <= 3 * 2 * 2.0 ** -11 + 1.2e-4
   o[0, 3, 5] = o[1, 69, 89] = 0
   assert (o == 0).all()
+
+
+@pytest.mark.parametrize('coeffs,steps', [
+  ((3.4445, -4.7750, 2.0315), 32), ((2.0, -0.045, 1e-4), 5), ((3.9, 0.0, 1e-6), 3), ((8.3, -23.6, 17.3), 2),
+  ((-2.0, -1.5, 0.5), 1)])
+def test_coefficients_that_fp16_holds(ops, coeffs, steps):
+  """Those near the limits are accepted, and nothing overflows: a rank-one matrix has
+  the singular value 1, the largest there is, here all of it in one entry x.  A step's own
+  error, of P = p(x^2): P - mu I and the first word of X are rounded to fp16 (mu between
+  1 and a), D's diagonal to second order, X to two words.  What the entry was off by
+  before grows by x (x p)' / (x p)."""
+  a, b, c = coeffs
+  x, off = 1.0, 2.0 ** -15
+  for _ in range(steps):
+    t = x * x
+    p, grows = a + b * t + c * t * t, a + 3 * b * t + 5 * c * t * t
+    own = 2 * 2.0 ** -11 * max(abs(p - a), abs(p - 1)) + abs(c) * ((t + b / (2 * c)) * 2.0 ** -11) ** 2
+    off = off * abs(grows / p) * (1 + 20 * off) + own / abs(p) + 2.0 ** -15
+    x *= p
+  g = torch.zeros(1, 140, 150, device='cuda')
+  g[0, 139, 7] = 5.0
+  o = move(ops, g, steps=steps, coeffs=coeffs)
+  assert o.isfinite().all() and (o != 0).sum() == 1
+  if steps < 8:      # the usual coefficients do not converge: 32 steps have no digit left
+    assert abs(o[0, 139, 7].item() / x - 1) <= off
+  full = ops.orthogonalize(torch.randn(1, 140, 150, device='cuda'), steps=steps, coeffs=coeffs)
+  assert full.isfinite().all()
