@@ -124,7 +124,9 @@ class Trainer:
                                 if entropy_weight is None else entropy_weight)
     if not math.isfinite(self.entropy_weight):
       raise ValueError(f'Trainer: entropy_weight={self.entropy_weight} must be finite')
-    self.last_entropy = None   # device scalar: mean entropy of the masked positions (entropy_weight != 0)
+    # device scalar: mean entropy of the masked (and attended) positions of the last
+    # forward_backward, 0 if there were none; None without the entropy term
+    self.last_entropy = None
     self.p_drop = float(bb.blocks[0].dropout if dropout is None else dropout)
     self.ema_decay = float(cfg.training.ema)
     # Two counters, as in the reference: `step_count` is the optimizer's (Adam bias
@@ -514,6 +516,7 @@ class Trainer:
     hfc, lgc, dlc = ws['hf'][:n_pad], ws['logits'][:n_pad], ws['dlogits'][:n_pad]
     weight = dsigma / torch.expm1(sigma)
     nlls = torch.zeros(B, L, dtype=torch.float32, device=self.dev)
+    self.last_entropy = torch.zeros((), device=self.dev) if self.entropy_weight else None
     if n_pad:
       sc = ws['scatter'][:n_pad].long()
       valid = sc >= 0
