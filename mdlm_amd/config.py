@@ -80,8 +80,10 @@ DEFAULTS = dict(
   training=dict(ema=0.9999, antithetic_sampling=True,
                 importance_sampling=False, sampling_eps=1e-3,
                 change_of_variables=False,
-                # mdlm_amd extension: the training loss is NELBO - entropy_weight * mean
-                # entropy of the masked positions' predictions (0: the reference's loss)
+                # mdlm_amd extension: the training loss is NELBO - entropy_weight * E (0: the
+                # reference's loss), E the entropies of the masked positions' predictions
+                # summed and divided by the number of attended positions, masked or not, as
+                # the NELBO is
                 entropy_weight=0.0),
   eval=dict(checkpoint_path='', disable_ema=False,
             compute_generative_perplexity=False, perplexity_batch_size=8,
