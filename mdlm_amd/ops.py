@@ -824,8 +824,8 @@ def muon_update(p, g, m, lr, ema=None, w16=None, momentum=0.95, weight_decay=0.0
     got = _matrices(t, name, (torch.bfloat16 if name == 'w16' else torch.float32,))
     if t.shape != p.shape or got != (n, r, c, ld, bs):
       raise RuntimeError(f'{name}: must have the shape and strides of p')
-  if sumsq is not None:
-    _dev(sumsq, 'sumsq', torch.float32)
+  if sumsq is not None and _dev(sumsq, 'sumsq', torch.float32).numel() == 0:
+    raise RuntimeError('sumsq: empty')
   if scale is None:
     scale = 0.2 * math.sqrt(max(r, c))
   if p.numel():
