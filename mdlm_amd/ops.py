@@ -40,6 +40,8 @@ def _rows2d(t, name):
     return t, t.shape[0], V, t.stride(0)
   if t.dim() == 3:
     B, L, _ = t.shape
+    if L == 1 and B > 1:     # one position of each sequence: stride(1) says nothing
+      return t, B, V, t.stride(0)
     ld = t.stride(1)
     if B > 1 and t.stride(0) != L * ld:
       raise RuntimeError(f'{name}: rows must be uniformly strided')

@@ -19,3 +19,27 @@ def test_muon_update_refuses_an_empty_norm(ops):
   with pytest.raises(RuntimeError, match='sumsq'):
     ops.muon_update(p, g, m, 1e-3, sumsq=torch.zeros(0, device='cuda'), max_norm=1.0)
   assert (p == 1).all() and (m == 1).all()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_one_position_of_each_sequence(ops, dtype):
+  """logits[:, i:i + 1] has rows at a constant distance, that of the sequences."""
+  B, L, V, mask = 3, 5, 1000, 999
+  gen = torch.Generator(device='cuda').manual_seed(0)
+  full = ops.alloc_logits(B, L, V, dtype)
+  full.copy_(torch.randn(B, L, V, generator=gen, device='cuda'))
+  one = full[:, 2:3]
+  x0 = torch.randint(0, V - 1, (B, 1), generator=gen, device='cuda')
+  xt = torch.full_like(x0, mask)
+  s = ops.subs_scores(one, xt, x0, mask, top_k=4)
+  want = ops.subs_scores(one.contiguous(), xt, x0, mask, top_k=4)
+  for got, ref in zip(s, want):
+    assert got.shape[:2] == (B, 1) and torch.equal(got, ref)
+  g = torch.rand(B, 1, generator=gen, device='cuda')
+  keep = full.clone()
+  d = ops.subs_scores_bwd(one, xt, x0, mask, s.lse, s.entropy, g_logp=g, g_entropy=g)
+  assert torch.equal(d, ops.subs_scores_bwd(one.contiguous(), xt, x0, mask, s.lse, s.entropy, g_logp=g, g_entropy=g))
+  ops.subs_scores_bwd(one, xt, x0, mask, s.lse, s.entropy, g_logp=g, g_entropy=g, dlogits=one)
+  assert torch.equal(one, d)
+  others = [i for i in range(L) if i != 2]
+  assert torch.equal(full[:, others], keep[:, others])
