@@ -9,19 +9,23 @@
 //   a + b t + c t^2 = c (t + b/2c)^2 + (a - b^2/4c),
 // D = A + (b/2c) I is small near convergence and nothing cancels:
 //   P = c D D^T + (a - b^2/4c) I,   X <- mu X + (P - mu I) X.
-// mu = a in the early steps (small singular values: P is close to a I), 1 in the last one
-// (P is close to I) and half way in the one before, when some values have arrived and some are
-// still small (1 there: 1.9e-3 instead of 1.1e-3 off for low rank and noise, 4096 x 8192, and
-// 20 % more on average over shapes and spectra).  The mu X term takes X from two words, fp16 and
-// e4m3 (15 bits together: 8 more bits of the second word take a decaying spectrum from 1.0e-3
-// to 9.6e-4, and it is a third of what the products move), so that only the small P - mu I
-// sees X rounded to fp16.  Without the second word matrices of fast decaying spectra lose: 1.2e-2.
-// The diagonal of D, its largest part, is also corrected for its rounding:
-// d = D_ii - fp16(D_ii) enters D D^T to first order.  Against 64 bits the result of five steps is
-// 3e-4 .. 1.3e-3 off (2-norm, relative; sides of up to 64 rows up to 1.6e-3, 16384 x 32768 with a
-// spectrum of i^-1.5 1.5e-3), less than rounding it to bf16 costs (1.7e-3); plain bf16 operands
-// are 1e-2 .. 3e-2 off.  The usual coefficients do not converge: a step more makes differences
-// larger (6 steps up to 2e-3, 7 3e-3, 10 1.5e-2), as it does to those of the input.
+// The mu X term takes X from two words, fp16 and e4m3 (15 bits together; 8 more bits of the
+// second word would take a spectrum of i^-1.5 from 4.2e-4 to 0.9e-4 at 4096 x 8192, less than the result's own
+// rounding shows, and it is a third of what the products move), so that only P - mu I sees X
+// rounded to fp16.  Without the second word matrices of fast decaying spectra lose: 1.2e-2.
+// Early, mu = a: P is a I but for the large singular values, the small ones are still multiplied by
+// a, and what P - a I makes of the rounding of X stays with the large ones.  In the last three
+// steps mu is each row's own P_ii (fp32), and P's off-diagonal part alone meets fp16.  (mu = 1 there:
+// twice the error, three times for low rank and noise.  P_ii in all steps: three times the error
+// for few rows of a decaying spectrum, 12 x 192, whose small values take on the roundings of the large.)
+// The diagonals of D and P, their largest parts, lose nothing to fp16: d = D_ii - fp16(D_ii)
+// enters D D^T to first order, and what fp16 leaves of P_ii - a goes to mu.
+//
+// Against 64 bits the result of five steps is 1e-4 .. 1.0e-3 off (2-norm, relative; fewer than 64
+// rows up to 2e-3, fewer than 8, hardly anything to average over, up to 8e-3; 16384 x 32768 with a
+// spectrum of i^-1.5 1.3e-3); rounding it to bf16 costs 1.7e-3; plain bf16 operands are 1e-2 .. 3e-2
+// off.  The usual coefficients do not converge: a step more makes differences larger, these as
+// well as the input's (6 steps up to 1.5e-3, 7 2.0e-3, 10 1.5e-2).
 //
 // Every matrix is padded with zeros to whole slabs of 64 in the workspace; padding
 // stays zero through every step.
@@ -44,8 +48,8 @@ constexpr float NS_SX = 2048.f;
 constexpr float NS_SD = 256.f;
 // Of the second word, what X loses in the first: at most 1 while the first is below 2^12, |X| < 2.
 // e4m3 goes from 2^-9 to 448, so 256 keeps the most of it that large matrices need, whose entries
-// are small (average of X_0 at 4096 x 8192: 0.35 with NS_SX).  Off by (decaying spectra, i^-1.5, of 1024 x 4096,
-// 4096 x 8192, 16384 x 32768) with 16: 2.0e-3, 4.6e-3, 1.0e-2, with 256: 1.0e-3, 1.0e-3, 1.7e-3.
+// are small (average of X_0 at 4096 x 8192: 0.35 with NS_SX).  Off by, with 16 / 256 (spectra of
+// i^-1.5): 1024 x 4096 1.8e-3 / 3.3e-4, 4096 x 8192 4.5e-3 / 4.2e-4, 8192 x 16384 7.4e-3 / 7.1e-4.
 constexpr float NS_SL = 256.f;
 constexpr float NS_LO_MAX = 448.f;    // larger X lose bits of the second word, no more
 
@@ -72,7 +76,7 @@ static inline NsShape ns_shape(int rows, int cols) {
 // workspace of n matrices
 struct NsWs {
   double* norm;      // n x NS_MAX_PARTS partial sums of squares
-  float* diag;       // n x sp
+  float *diag, *mu;  // n x sp
   f16* h[2];         // n x sp x lp, X's first words
   uint8_t* lo;       // n x sp x lp, its second words
   f16 *d, *p;        // n x sp x sp, or
@@ -89,12 +93,14 @@ static inline int64_t ns_layout(const NsShape& q, int n, char* base, NsWs* w) {
   t.h[1] = (f16*)take(x * 2);
   t.lo = (uint8_t*)take(x);
   t.d = t.p = nullptr;
+  t.mu = nullptr;
   t.part = nullptr;
   if (q.sp <= NS_SMALL) {
     t.part = (float*)take(d * q.splits * 4);
   } else {
     t.d = (f16*)take(d * 2);
     t.p = (f16*)take(d * 2);
+    t.mu = (float*)take((int64_t)n * q.sp * 4);
   }
   if (w) *w = t;
   return off;
@@ -358,8 +364,10 @@ struct NsGemm {
   f16* out; int64_t ldo, bso;        // D, P or the next X's high words
   uint8_t* lo;                       // APPLY: X's second words, in place
   float* diag; int sp;               // rounding of D's diagonal
+  float* row_mu;                     // what a row of X's two words is multiplied by
   float* part; int splits;           // GRAM: sums of so many parts of K go here as they are (null: D is made of one)
-  float shift, c, mu;                // see the head of this file
+  float shift, c, mu, p0;            // see the head of this file; p0 = a - b^2/4c - mu
+  int own;                           // P's diagonal goes to row_mu whole, not its rounding alone
   int last, tall;                    // APPLY: the result goes to dst
   NsOut dst;
 };
@@ -405,7 +413,26 @@ struct NsTile {
   // where registers allow (64-tiles: few of them run and each waits for its own
   // latency), else before the sums are turned round.
   static constexpr bool EARLY = T == 64;
-  struct Fetched { f16x8 x[NC]; uint2 lo[NC]; float di[EARLY ? NC : 1]; f32x4 dj[EARLY ? NC : 1][2]; bool ok[NC]; };
+  struct Fetched {
+    f16x8 x[NC]; uint2 lo[NC]; bool ok[NC];
+    float di[EARLY || MODE == NS_APPLY ? NC : 1];      // of the row: rounding of D's diagonal, or mu
+    f32x4 dj[EARLY ? NC : 1][2];
+  };
+  static __device__ __forceinline__ void fetch_mu(const NsGemm& g, int b, int ip, Fetched& f) {
+    if constexpr (MODE == NS_APPLY) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        if (f.ok[c]) f.di[c] = g.row_mu[b * g.sp + ip + (threadIdx.x + c * THREADS) / CH];
+    }
+  }
+  // One element of P's diagonal, P_ii - mu times NS_SD: what goes into P as fp16, and the
+  // rest, to which X's two words are multiplied.
+  static __device__ __forceinline__ float split_diag(const NsGemm& g, float q, float& row_mu) {
+    q = pinned(q);
+    const float in_p = g.own ? 0.f : (float)(f16)q;
+    row_mu = __builtin_fmaf(q - in_p, 1.f / NS_SD, g.mu);
+    return in_p;
+  }
   static __device__ __forceinline__ void fetch(const NsGemm& g, int b, int i0, int ip, int j0, Fetched& f) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
@@ -474,7 +501,7 @@ struct NsTile {
     for (int part = 0; part < T / ER; ++part) {
       const int ip = i0 + part * ER;
       Fetched late;
-      if (!EARLY) fetch(g, b, i0, ip, j0, late);
+      if (!EARLY) { fetch(g, b, i0, ip, j0, late); fetch_mu(g, b, ip, late); }
       const Fetched& f = EARLY ? early : late;
       __syncthreads();
       if (T == ER || wr * TM / ER == part) {
@@ -523,7 +550,12 @@ struct NsTile {
             x[e] = (x[e] + (di + (e < 4 ? d0[e & 3] : d1[e & 3])) * (float)f.x[c][e]) * (g.c / NS_SD);
           if (on_diag >= 0 && on_diag < 8) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) if (e == on_diag) x[e] += g.mu * NS_SD;      // (a - b^2/4c) - mu
+            for (int e = 0; e < 8; ++e)
+              if (e == on_diag) {
+                float m;
+                x[e] = split_diag(g, x[e] + g.p0 * NS_SD, m);
+                g.row_mu[b * g.sp + i] = m;
+              }
           }
         } else {
           const float sc = g.last ? 1.f / NS_SX : 1.f;
@@ -531,7 +563,7 @@ struct NsTile {
           unpack_fp8(f.lo[c], l8);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            x[e] = (g.mu * __builtin_fmaf(l8[e], 1.f / NS_SL, (float)f.x[c][e]) + x[e] * (1.f / NS_SD)) * sc;
+            x[e] = (f.di[c] * __builtin_fmaf(l8[e], 1.f / NS_SL, (float)f.x[c][e]) + x[e] * (1.f / NS_SD)) * sc;
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = pinned(x[e]);
@@ -619,7 +651,7 @@ struct NsTile {
     unsigned tr[FN];
     if constexpr (MODE == NS_APPLY) tr_setup(smem + OP, wc, lane, tr);
     Fetched early;
-    if (EARLY) fetch(g, b, i0, i0, j0, early);
+    if (EARLY) { fetch(g, b, i0, i0, j0, early); fetch_mu(g, b, i0, early); }
     f32x4 acc[FM][FN];
 #pragma unroll
     for (int m = 0; m < FM; ++m)
@@ -750,7 +782,7 @@ __global__ __launch_bounds__(64 * WM * WN, T <= 128 ? 2 : WM * WN / 4) void ns_g
 // parts that GRAM left, makes 64 rows of P in LDS and multiplies `group` 64 x 64 tiles of X
 // by them, the next one's X on its way meanwhile.  LDS rows as in NsTile.
 template <int S>
-__global__ __launch_bounds__(256) void ns_step_kernel(NsGemm g, float p_diag, int group) {
+__global__ __launch_bounds__(256) void ns_step_kernel(NsGemm g, int group) {
   using Tile = NsTile<NS_APPLY, 64, 2, 2, 4>;
   constexpr int KS = S / 64, DSLAB = S * 128, SLAB = 64 * 128;
   // D; later the epilogue's tile and X's second buffer
@@ -759,6 +791,7 @@ __global__ __launch_bounds__(256) void ns_step_kernel(NsGemm g, float p_diag, in
   __shared__ __attribute__((aligned(16))) char xs[KS * SLAB];
   __shared__ __attribute__((aligned(16))) char ps[KS * SLAB];
   __shared__ __attribute__((aligned(16))) float diag[S];
+  __shared__ float row_mu[64];
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wid >> 1, wc = wid & 1, fr = lane & 15, fq = lane >> 4;
   const int tiles_n = g.N / 64, per_mat = KS * ((tiles_n + group - 1) / group), total = per_mat * g.n, per_xcd = (total + 7) >> 3;
@@ -844,13 +877,15 @@ __global__ __launch_bounds__(256) void ns_step_kernel(NsGemm g, float p_diag, in
         const f16x4 d = *reinterpret_cast<const f16x4*>(dm + at(i, j, DSLAB));
         const float di = diag[i];
         const f32x4 dj = *reinterpret_cast<const f32x4*>(diag + j);
-        f16x4 h;
+        float x[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x = (acc[m][n][e] + (di + dj[e]) * (float)d[e]) * (g.c / NS_SD);
-          if (i == j + e) x += p_diag * NS_SD;
-          h[e] = (f16)x;
+        for (int e = 0; e < 4; ++e) x[e] = (acc[m][n][e] + (di + dj[e]) * (float)d[e]) * (g.c / NS_SD);
+        if (i0 + wr * 32 + m * 16 == wc * (S / 2) + n * 16) {      // one branch per wave
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i == j + e) x[e] = Tile::split_diag(g, x[e] + g.p0 * NS_SD, row_mu[r]);
         }
+        const f16x4 h = {(f16)x[0], (f16)x[1], (f16)x[2], (f16)x[3]};
         *reinterpret_cast<f16x4*>(ps + at(r, j, SLAB)) = h;
       }
   }
@@ -885,11 +920,13 @@ __global__ __launch_bounds__(256) void ns_step_kernel(NsGemm g, float p_diag, in
             acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf[ks][n], fa, acc[m][n], 0, 0, 0);
         }
     }
+#pragma unroll
+    for (int c = 0; c < Tile::NC; ++c) own.di[c] = row_mu[(tid + c * Tile::THREADS) / Tile::CH];
     Tile::finish(g, b, tm, tn, 0, own, acc, dm);
     own = next;
   }
 }
-static int ns_step(const NsGemm& g, float p_diag, int cus, hipStream_t st) {
+static int ns_step(const NsGemm& g, int cus, hipStream_t st) {
   // as many tiles per workgroup as leave two workgroups per CU (what LDS has room for); us per
   // call with one tile each / four workgroups per CU / two / one: 64 x 128 x 2048:
   // 405 / 228 / 204 / 234, 4 x 128 x 8192: 177 / 167 / 131 / 131
@@ -899,8 +936,8 @@ static int ns_step(const NsGemm& g, float p_diag, int cus, hipStream_t st) {
   const int64_t total = (int64_t)(g.M / 64) * ((tiles_n + group - 1) / group) * g.n;
   if (total >= (1ll << 28)) { set_error("orthogonalize: too many tiles"); return -1; }
   const unsigned grid = (unsigned)((total + 7) / 8 * 8);
-  if (g.M == 64) ns_step_kernel<64><<<grid, 256, 0, st>>>(g, p_diag, (int)group);
-  else ns_step_kernel<128><<<grid, 256, 0, st>>>(g, p_diag, (int)group);
+  if (g.M == 64) ns_step_kernel<64><<<grid, 256, 0, st>>>(g, (int)group);
+  else ns_step_kernel<128><<<grid, 256, 0, st>>>(g, (int)group);
   MDLM_LAUNCH_CHECK();
   return 0;
 }
@@ -957,7 +994,7 @@ static int ns_gemm(const NsGemm& g, int cus, hipStream_t st) {
 }
 
 static inline double ns_mu(int it, int steps, double a) {
-  return it + 2 < steps ? a : it + 2 == steps ? 0.5 * (a + 1.0) : 1.0;
+  return it + 3 < steps ? a : 1.0;
 }
 // Whether X, D and P - mu I stay in the range of fp16 with their scales, whatever the matrix:
 // an entry is at most the largest singular value, X_0's are in [0, 1], and each step maps [0, s]
@@ -1007,20 +1044,20 @@ static int ns_run(NsSrc src, NsOut dst, int n, int rows, int cols, int steps, do
     const double mu = ns_mu(it, steps, a);
     f16 *x = w.h[it & 1], *xn = w.h[(it & 1) ^ 1];
     NsGemm g = {};
-    g.n = n; g.sp = q.sp; g.diag = w.diag; g.part = w.part; g.splits = q.splits;
+    g.n = n; g.sp = q.sp; g.diag = w.diag; g.row_mu = w.mu; g.part = w.part; g.splits = q.splits;
+    g.mu = (float)mu; g.p0 = (float)(a - b * b / (4 * c) - mu); g.own = it + 3 >= steps;
     g.A = x; g.lda = q.lp; g.bsa = bx; g.B = x; g.ldb = q.lp; g.bsb = bx; g.K = q.lp;
     g.M = g.N = q.sp;
     g.out = w.d; g.ldo = q.sp; g.bso = bd; g.shift = (float)(b / (2 * c));
-    const float p_diag = (float)(a - b * b / (4 * c) - mu);
     if (int rc = w.part ? ns_launch<NS_GRAM, 64, 2, 2, 4>(g, st) : ns_gemm<NS_GRAM>(g, cus, st)) return rc;
     g.A = w.d; g.lda = q.sp; g.bsa = bd; g.B = w.d; g.ldb = q.sp; g.bsb = bd; g.K = q.sp;
-    g.out = w.p; g.c = (float)c; g.mu = p_diag;
+    g.out = w.p; g.c = (float)c;
     if (!w.part)
       if (int rc = ns_gemm<NS_SQUARE>(g, cus, st)) return rc;
     g.A = w.p; g.B = x; g.ldb = q.lp; g.bsb = bx; g.N = q.lp;
-    g.out = xn; g.ldo = q.lp; g.bso = bx; g.lo = w.lo; g.mu = (float)mu;
+    g.out = xn; g.ldo = q.lp; g.bso = bx; g.lo = w.lo;
     g.last = it + 1 == steps; g.tall = q.tall; g.dst = dst;
-    if (int rc = w.part ? ns_step(g, p_diag, cus, st) : ns_gemm<NS_APPLY>(g, cus, st)) return rc;
+    if (int rc = w.part ? ns_step(g, cus, st) : ns_gemm<NS_APPLY>(g, cus, st)) return rc;
   }
   return 0;
 }

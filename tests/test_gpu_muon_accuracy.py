@@ -75,3 +75,38 @@ def low_rank(r, c, seed=0):
 @pytest.mark.parametrize('r,c', [(256, 512), (128, 1024), (1024, 4096), (8192, 2048), (4096, 8192)])
 def test_low_rank_and_noise(ops, r, c):
   check(ops, low_rank(r, c))
+
+
+@pytest.mark.parametrize('steps', [1, 2, 3, 5])
+@pytest.mark.parametrize('n,r,k', [(2, 24, 7), (1, 128, 3), (1, 300, 4), (3, 150, 64)])
+def test_equal_singular_values(ops, n, r, k, steps):
+  """Rows that do not meet, each k columns of its own, all of one length: every product
+  is diagonal, and an element x sees what is lost on the diagonals.  D's rounding enters to
+  second order, X is held in two words, and P is exact but for fp32; in steps before the last
+  three the first word of X alone meets P - a.  A is made of the first words alone: of a sum of
+  squares t each term is off by at most 2 x 2^-11, and P = a + b t + c t^2 by |b t + 2 c t^2| times
+  that.  What a row was off by before grows by x (x p)' / (x p).  With P - mu I rounded to
+  fp16 one step loses up to 7e-4, and one or two steps more than the bound in all of these
+  shapes."""
+  gen = torch.Generator(device='cuda').manual_seed(r)
+  rows = torch.randn(n, r, k, generator=gen, device='cuda').double()
+  rows = rows / rows.norm(dim=2, keepdim=True)
+  g = torch.zeros(n, r, r, k, device='cuda')
+  g[:, range(r), range(r)] = rows.float()
+  s, off, floor = r ** -0.5, 2.0 ** -15, 2.0 ** -29
+  for it in range(steps):
+    t = s * s
+    p, grows = A + B * t + C * t * t, A + 3 * B * t + 5 * C * t * t
+    own = C * ((t + B / (2 * C)) * 2.0 ** -11) ** 2 + 16 * 2.0 ** -24 * A
+    own += 2 * 2.0 ** -11 * abs(B * t + 2 * C * t * t)
+    if it + 3 < steps:
+      own += 2.0 ** -11 * abs(p - A)
+    off = off * max(1.0, abs(grows / p)) * (1 + 10 * off) + own / abs(p) + 2.0 ** -15
+    floor = floor * max(abs(p), abs(grows)) + 2.0 ** -29
+    s *= p
+  want = torch.zeros(n, r, r, k, dtype=torch.float64, device='cuda')
+  want[:, range(r), range(r)] = rows * s
+  for got in (move(ops, g.view(n, r, r * k), steps=steps),
+              move(ops, g.view(n, r, r * k).transpose(1, 2).contiguous(), steps=steps).transpose(1, 2)):
+    err = (got.reshape(n, r, r, k).double() - want).abs()
+    assert (err <= off * want.abs() + floor).all(), ((err - floor) / want.abs()).nan_to_num(0).max().item() / off
