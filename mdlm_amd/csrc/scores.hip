@@ -294,10 +294,15 @@ __global__ __launch_bounds__(BLOCK) void subs_scores_kernel(
   float off = __builtin_fmaf(m, SC_L2E, -m2);        // what the rounding of m2 moved s by
   const bool plain = s > 0.f;                        // workgroup-uniform; false for NaN too
   if (!plain) { slow_stats<T, BLOCK>(row, V, mask, sh, m, s, s1); off = 0.f; }
-  const float l2s = log2f(s), lz = (l2s - off) * SC_LN2;
+  // log Z and the entropy are not below 0, but for what the logarithm rounds where one token
+  // has all the weight (NaN stays NaN)
+  const float l2s = log2f(s);
+  float lz = (l2s - off) * SC_LN2;
+  if (lz < 0.f) lz = 0.f;
   if (tid == 0) {
+    const float h = (l2s - s1 / s) * SC_LN2;
     lse[r] = m + lz;
-    ent[r] = (l2s - s1 / s) * SC_LN2;
+    ent[r] = h < 0.f ? 0.f : h;
     // a row without a finite logit has no scores, not even the mask token's
     logp[r] = tgt < 0 || tgt >= V ? 0.f
               : m == -INFINITY   ? NAN

@@ -43,3 +43,19 @@ def test_one_position_of_each_sequence(ops, dtype):
   assert torch.equal(one, d)
   others = [i for i in range(L) if i != 2]
   assert torch.equal(full[:, others], keep[:, others])
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('rows,V', [(200, 9000), (3000, 500), (7, 3)])
+def test_scores_of_certain_tokens(ops, rows, V, dtype):
+  """One token has (nearly) all the weight: its log-probability is not above 0, nor the
+  entropy below it, whatever the logits' size."""
+  gen = torch.Generator(device='cuda').manual_seed(V)
+  mask = V - 1
+  x = torch.randn(rows, V, generator=gen, device='cuda')
+  top = torch.randint(0, mask, (rows,), generator=gen, device='cuda')
+  x[torch.arange(rows, device='cuda'), top] += 10 + 2000 * torch.rand(rows, generator=gen, device='cuda') ** 3
+  x += 3000 * torch.rand(rows, 1, generator=gen, device='cuda') ** 2
+  xt = torch.full_like(top, mask)
+  s = ops.subs_scores(x.to(dtype), xt, top, mask, top_k=2)
+  assert (s.logp <= 0).all() and (s.top_logp <= 0).all() and (s.entropy >= 0).all()
