@@ -103,6 +103,13 @@ template <> __device__ __forceinline__ void unpack16<bf16_t, float[8]>(const uin
 // m starts at a finite value below every logit that counts, so that no infinity
 // meets another; a row with nothing above it goes the slow way.
 constexpr float SC_FLOOR = -1e30f;
+// m2.  Rounded before any use: the compiler would fold the product into the differences of two m2,
+// and what the sums were made with no longer cancels (1.2e-4 in a log-probability at logits of 1e4).
+__device__ __forceinline__ float max_log2(float m) {
+  float m2 = m * SC_L2E;
+  asm("" : "+v"(m2));
+  return m2;
+}
 struct Running {
   float m = SC_FLOOR, m2 = SC_FLOOR * SC_L2E, s = 0.f, s1 = 0.f;
   float next = SC_FLOOR;        // the largest maximum of any other chunk than `best`, which holds m
@@ -115,7 +122,7 @@ struct Running {
     next = fmaxf(next, fminf(m, mx));
     if (mx > m) {
       best = chunk;
-      const float n2 = mx * SC_L2E, d = m2 - n2, sc = __builtin_amdgcn_exp2f(d);
+      const float n2 = max_log2(mx), d = m2 - n2, sc = __builtin_amdgcn_exp2f(d);
       s1 = __builtin_fmaf(d, s, s1) * sc;
       s *= sc;
       m = mx; m2 = n2;
@@ -265,7 +272,7 @@ __global__ __launch_bounds__(BLOCK) void subs_scores_kernel(
   }
   // ---- across the workgroup
   const float own = run.m;
-  const float wm = wave_max(own), wm2 = wm * SC_L2E;
+  const float wm = wave_max(own), wm2 = max_log2(wm);
   float s, s1;
   {
     const float d = run.m2 - wm2, sc = __builtin_amdgcn_exp2f(d);
@@ -283,11 +290,11 @@ __global__ __launch_bounds__(BLOCK) void subs_scores_kernel(
   float m = sh.m[0];
 #pragma unroll
   for (int j = 1; j < BLOCK / 64; ++j) m = fmaxf(m, sh.m[j]);
-  const float m2 = m * SC_L2E;
+  const float m2 = max_log2(m);
   s = s1 = 0.f;
 #pragma unroll
   for (int j = 0; j < BLOCK / 64; ++j) {
-    const float d = sh.m[j] * SC_L2E - m2, sc = __builtin_amdgcn_exp2f(d);
+    const float d = max_log2(sh.m[j]) - m2, sc = __builtin_amdgcn_exp2f(d);
     s1 += __builtin_fmaf(d, sh.s[j], sh.s1[j]) * sc;
     s += sh.s[j] * sc;
   }
