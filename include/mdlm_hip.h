@@ -553,11 +553,15 @@ int mdlm_subs_scores_bwd(const void* logits, int64_t ld, int dtype,
  * X <- a X + (b A + c A^2) X with A = X X^T (X^T X for a tall G): singular values
  * go towards 1, singular vectors stay.  No reference counterpart (its optimizer
  * is AdamW, diffusion.py:449-459).  n matrices (rows, cols), fp32 or bf16, rows
- * `ld` and matrices `stride` elements apart; out bf16 (the products round their
- * operands to fp16: the result is good to bf16).  |a| <= 16, 0 < |c| <= 32, |b^2 / 4c| <= 16,
- * steps <= 32, and coefficients that take a singular value from [0, 1] past 31 before the last
- * step, or its square t, |t + b / 2c| or |a + b t + c t^2 - 1| past 248, are refused (fp16
- * holds no more); |G|_F + eps counts as at least 6.1e-36.
+ * `ld` and matrices `stride` elements apart; out bf16.
+ * The products round their operands to fp16 (X itself is kept in 15 bits): with
+ * the usual coefficients and 5 steps the result is 1e-4 .. 1e-3 off in the 2-norm
+ * before it is rounded to bf16, 2e-3 for sides of less than 64, 8e-3 of less than
+ * 8; every step past the sixth enlarges that.
+ * Refused: |a| > 16, c = 0, |c| > 32, |b^2 / 4c| > 16, steps > 32, and coefficients
+ * that take a singular value from [0, 1] past 31 before the last step, or its square
+ * t, |t + b / 2c| or |a + b t + c t^2 - 1| past 248 (fp16 holds no more).
+ * |G|_F + eps counts as at least 6.1e-36.
  * `out` may be g itself.  ws: mdlm_orthogonalize_workspace_bytes(n, rows, cols),
  * 256-byte aligned; calls that overlap in time (two streams, two captured graphs
  * replayed at once) need one each. */
@@ -573,6 +577,8 @@ int mdlm_orthogonalize(const void* g, int64_t ldg, int64_t g_stride, int dtype,
  *   m <- m + (1 - momentum) (g - m)
  *   O  = orthogonalize(g + momentum (m - g))
  *   p <- p (1 - lr weight_decay) - lr update_scale O
+ * O is not rounded to bf16 here, and as accurate as stated there: the move of the
+ * fp32 weights is good to 10 bits or so, not to fp32.
  * p, g, m, ema (may be NULL): fp32, w_bf16 (may be NULL): bf16, all of the same
  * layout (rows `ld`, matrices `stride` elements apart).  g is not written.
  * The buffers must not overlap.  ws: as mdlm_orthogonalize. */

@@ -22,7 +22,8 @@
 // enters D D^T to first order, and what fp16 leaves of P_ii - a goes to mu.
 //
 // Against 64 bits the result of five steps is 1e-4 .. 1.0e-3 off (2-norm, relative; fewer than 64
-// rows up to 2e-3, fewer than 8, hardly anything to average over, up to 8e-3; 16384 x 32768 with a
+// rows up to 2e-3, fewer than 8, hardly anything to average over, up to 8e-3 (and bf16's own 2^-8 of
+// an element with that: 1.3e-2); 16384 x 32768 with a
 // spectrum of i^-1.5 1.3e-3); rounding it to bf16 costs 1.7e-3; plain bf16 operands are 1e-2 .. 3e-2
 // off.  The usual coefficients do not converge: a step more makes differences larger, these as
 // well as the input's (6 steps up to 1.5e-3, 7 2.0e-3, 10 1.5e-2).
@@ -778,7 +779,8 @@ __global__ __launch_bounds__(64 * WM * WN, T <= 128 ? 2 : WM * WN / 4) void ns_g
 // SQUARE and APPLY of matrices whose short side fits into 128 rows, in one launch: a
 // launch costs 4 us there, the products next to nothing (us per call, three launches per
 // step / two: 2 x 384 x 128: 67 / 60, 128 x 4096: 124 / 81, 16 x 6000: 141 / 67,
-// 300 x 100 x 140: 202 / 174, 64 x 128 x 2048: 200 / 204).  Every workgroup sums D from the
+// 300 x 100 x 140: 202 / 174, 64 x 128 x 2048: 200 / 204; before P's diagonal went to mu, which costs
+// 1 .. 4 %: 63, 83, 70, 181, 200 now).  Every workgroup sums D from the
 // parts that GRAM left, makes 64 rows of P in LDS and multiplies `group` 64 x 64 tiles of X
 // by them, the next one's X on its way meanwhile.  LDS rows as in NsTile.
 template <int S>
