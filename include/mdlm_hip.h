@@ -553,7 +553,8 @@ int mdlm_subs_scores_bwd(const void* logits, int64_t ld, int dtype,
  * X <- a X + (b A + c A^2) X with A = X X^T (X^T X for a tall G): singular values
  * go towards 1, singular vectors stay.  No reference counterpart (its optimizer
  * is AdamW, diffusion.py:449-459).  n matrices (rows, cols), fp32 or bf16, rows
- * `ld` and matrices `stride` elements apart; out bf16.
+ * `ld` and matrices `stride` elements apart (behind one another, or side by side within
+ * a row); out bf16.
  * The products round their operands to fp16 (X itself is kept in 15 bits): with
  * the usual coefficients and 5 steps the result is 1e-4 .. 1e-3 off in the 2-norm
  * before it is rounded to bf16, 2e-3 for sides of less than 64, 8e-3 of less than

@@ -1070,7 +1070,10 @@ static int ns_check(const char* who, int n, int rows, int cols, int64_t ld, int6
   MDLM_CHECK_ARG(n > 0 && n < 65536 && rows > 0 && cols > 0 && rows <= (1 << 17) && cols <= (1 << 17),
                  "%s: bad shape", who);
   MDLM_CHECK_ARG((rows < cols ? rows : cols) <= (1 << 15), "%s: the smaller side must be at most 32768", who);
-  MDLM_CHECK_ARG(ld >= cols && (n == 1 || bs >= (int64_t)(rows - 1) * ld + cols), "%s: overlapping rows or matrices", who);
+  // one matrix behind the other, or side by side within a row
+  MDLM_CHECK_ARG(ld >= cols && (n == 1 || bs >= (int64_t)(rows - 1) * ld + cols ||
+                                (bs >= cols && ld >= (int64_t)(n - 1) * bs + cols)),
+                 "%s: overlapping rows or matrices", who);
   MDLM_CHECK_ARG(steps >= 1 && steps <= 32, "%s: steps=%d is outside 1..32", who, steps);
   // the completed square's constant is what rounding D costs: 2.8 for the usual coefficients
   MDLM_CHECK_ARG(isfinite(a) && isfinite(b) && isfinite(c) && fabs(a) <= 16 && c != 0.0 && fabs(c) <= 32 &&

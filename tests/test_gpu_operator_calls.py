@@ -59,3 +59,25 @@ def test_scores_of_certain_tokens(ops, rows, V, dtype):
   xt = torch.full_like(top, mask)
   s = ops.subs_scores(x.to(dtype), xt, top, mask, top_k=2)
   assert (s.logp <= 0).all() and (s.top_logp <= 0).all() and (s.entropy >= 0).all()
+
+
+def test_matrices_side_by_side(ops):
+  """Column blocks of one wide matrix as a stack: they do not overlap."""
+  n, r, c = 3, 70, 132
+  gen = torch.Generator(device='cuda').manual_seed(5)
+  flat = {k: torch.randn(r, 20 + n * c, generator=gen, device='cuda') * 0.1 for k in 'pgme'}
+  flat['w'] = flat['p'].bfloat16()
+  keep = {k: t.clone() for k, t in flat.items()}
+  side = {k: t[:, 20:].view(r, n, c).transpose(0, 1) for k, t in flat.items()}
+  apart = {k: t.contiguous() for k, t in side.items()}
+  assert torch.equal(ops.orthogonalize(side['g']), ops.orthogonalize(apart['g']))
+  out = torch.zeros(r, n * c, dtype=torch.bfloat16, device='cuda')
+  ops.orthogonalize(apart['g'], out=out.view(r, n, c).transpose(0, 1))
+  assert torch.equal(out.view(r, n, c).transpose(0, 1), ops.orthogonalize(apart['g']))
+  for v in (side, apart):
+    ops.muon_update(v['p'], v['g'], v['m'], 1e-2, ema=v['e'], w16=v['w'], ema_one_minus_decay=0.1)
+  assert all(torch.equal(side[k], apart[k]) for k in side)
+  assert all(torch.equal(flat[k][:, :20], keep[k][:, :20]) for k in flat) and not torch.equal(side['p'][2], keep['p'][:, -c:])
+  for stride in (c - 1, 0):        # these do
+    with pytest.raises(RuntimeError, match='overlapping'):
+      ops.orthogonalize(flat['g'].as_strided((2, r, c), (stride, 20 + n * c, 1)))
