@@ -41,6 +41,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int NS_BK = 64;
+constexpr int NS_MAX_SIDE = 32768;    // the smaller one
 constexpr int NS_MAX_PARTS = 1024;    // partial sums of |G|^2 per matrix, at most
 // Powers of two that keep the fp16 words away from the subnormal range: entries
 // of X are at most about 1.2 and about 1/sqrt(s l) on average, D and P are at
@@ -1069,7 +1070,7 @@ static int ns_check(const char* who, int n, int rows, int cols, int64_t ld, int6
                     double c, double eps) {
   MDLM_CHECK_ARG(n > 0 && n < 65536 && rows > 0 && cols > 0 && rows <= (1 << 17) && cols <= (1 << 17),
                  "%s: bad shape", who);
-  MDLM_CHECK_ARG((rows < cols ? rows : cols) <= (1 << 15), "%s: the smaller side must be at most 32768", who);
+  MDLM_CHECK_ARG((rows < cols ? rows : cols) <= NS_MAX_SIDE, "%s: the smaller side must be at most %d", who, NS_MAX_SIDE);
   // one matrix behind the other, or side by side within a row
   MDLM_CHECK_ARG(ld >= cols && (n == 1 || bs >= (int64_t)(rows - 1) * ld + cols ||
                                 (bs >= cols && ld >= (int64_t)(n - 1) * bs + cols)),
@@ -1090,7 +1091,9 @@ static int ns_check(const char* who, int n, int rows, int cols, int64_t ld, int6
 using namespace mdlm;
 
 extern "C" int64_t mdlm_orthogonalize_workspace_bytes(int n, int rows, int cols) {
-  if (n <= 0 || rows <= 0 || cols <= 0 || n >= 65536 || rows > (1 << 17) || cols > (1 << 17)) return -1;
+  if (n <= 0 || rows <= 0 || cols <= 0 || n >= 65536 || rows > (1 << 17) || cols > (1 << 17) ||
+      (rows < cols ? rows : cols) > NS_MAX_SIDE)
+    return -1;
   return ns_layout(ns_shape(rows, cols), n, nullptr, nullptr);
 }
 

@@ -1,6 +1,7 @@
 """CPU-only checks of the orthogonalised update beyond test_operators_host.py."""
 import pytest
 
+from mdlm_amd import ops
 from test_operators_host import _muon, _ortho
 
 
@@ -18,3 +19,13 @@ def test_coefficients_past_fp16_are_refused(coeffs, steps):
   for call in (_ortho, _muon):
     with pytest.raises(RuntimeError, match='coefficients .* fp16'):
       call(steps=steps, **dict(zip('abc', coeffs)))
+
+
+def test_workspace_query_refuses_what_the_call_refuses():
+  """No workspace of many gigabytes for a call that would not run."""
+  assert ops.workspace_bytes('orthogonalize', 1, 32768, 40000) > 0
+  for rows, cols in ((32769, 40000), (131072, 32769)):
+    with pytest.raises(RuntimeError, match='bad shape'):
+      ops.workspace_bytes('orthogonalize', 1, rows, cols)
+    with pytest.raises(RuntimeError, match='smaller side'):
+      _ortho(n=1, rows=rows, cols=cols, ldg=cols, ldo=cols)
